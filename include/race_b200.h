@@ -317,6 +317,127 @@ int race_forward_static(const race_desc_t* desc, race_tensor_t q, race_tensor_t 
                         race_tensor_t v, const float* planes, const float* scale,
                         race_tensor_t out, cudaStream_t stream);
 
+/* ---- 8-bit operators around the attention --------------------------------
+ * What a block of RACE layers runs next to the attention when its linear
+ * layers are held in 8 bits: a root-mean-square norm with the residual's
+ * addition, quantisation with one scale for each 128 elements, the matrix
+ * product of such operands, and the optimizer step.  The reference runs these
+ * as torch modules in 32 bits (nn.LayerNorm / nn.Linear in misc/vit.py:1040-1068
+ * and misc/race.py:176-206, torch.optim.AdamW in its training drivers).
+ *
+ * A value is its 8-bit code (4 exponent bits, 3 mantissa bits, no infinity,
+ * largest 448) times the float32 scale of its block.  A block's scale is
+ * s = max(amax * (1/448), 2^-126), amax its largest magnitude, and a code is
+ * x * (1 / s) rounded to nearest even (each step in float32); a block that holds an infinity or a NaN
+ * gets a non-finite scale, so that everything it enters shows it. */
+
+/* Rows of elements; `ld` elements between rows, columns contiguous. */
+typedef struct {
+  void* data;
+  int64_t ld;
+} race_rows_t;
+
+/* 8-bit codes with their scales: code (r, c) at codes[r * ld + c] (codes and ld
+ * multiples of 16 bytes), the scale of row (or, for square blocks, row block)
+ * i and column block j at scales[i * stride_row + j * stride_block].  Rows that
+ * are summed over by the product should have stride_row = 1: the tiles then
+ * read their scales in whole lines. */
+typedef struct {
+  void* codes;
+  int64_t ld;
+  float* scales;
+  int64_t stride_row, stride_block;
+} race_blocks_t;
+
+/* Quantises x [rows][cols] (race_dtype_t dtype).  square = 0: one scale for
+ * each 128 columns of a row in by_rows, and one for each 128 rows of a column
+ * in by_cols, which receives x transposed ([cols][rows]).  square = 1: one
+ * scale for each 128 x 128 block; by_cols receives the same codes transposed,
+ * and its scales ([column block][row block]) where by_cols.scales is given.
+ * Either output may be left out (codes = NULL), not both.  Bytes between the
+ * last column of by_rows (the last row in by_cols) and the next multiple of 16
+ * are set to zero. */
+int race_quantize(race_rows_t x, int32_t dtype, int64_t rows, int64_t cols, int32_t square,
+                  race_blocks_t by_rows, race_blocks_t by_cols, cudaStream_t stream);
+
+typedef struct {
+  int32_t dtype;          /* race_dtype_t of x, residual, h, y and their gradients */
+  int32_t weight_dtype;   /* race_dtype_t of the weight and its gradient           */
+  int64_t rows;
+  int64_t width;          /* 1 to 65536                                            */
+  float eps;
+} race_norm_desc_t;
+
+/* h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, row by row in 32
+ * bits.  residual may be NULL (then h = x and is not written); h is rounded to
+ * dtype when it is stored, y is formed from the sum before that rounding.
+ * y: dtype, or NULL with y8 given (8-bit codes, one scale for each 128
+ * columns).  rstd: optional [rows], 1 / sqrt(mean(h^2) + eps), which the
+ * backward pass reads. */
+int race_rms_norm(const race_norm_desc_t* desc, race_rows_t x, race_rows_t residual,
+                  const void* weight, race_rows_t y, race_blocks_t y8, race_rows_t h, float* rstd,
+                  cudaStream_t stream);
+/* Workspace bytes of race_rms_norm_backward (partial sums of dweight). */
+size_t race_rms_norm_workspace(const race_norm_desc_t* desc);
+/* g = dy * weight; dx = dh + rstd * (g - h * rstd^2 * mean(g * h)) (the gradient
+ * of x and of the residual alike), dweight = sum over rows of dy * h * rstd.
+ * dh: the gradient that reaches h by itself, or NULL.  Sums are taken in a
+ * fixed order. */
+int race_rms_norm_backward(const race_norm_desc_t* desc, race_rows_t dy, race_rows_t dh,
+                           race_rows_t h, const void* weight, const float* rstd, race_rows_t dx,
+                           void* dweight, void* workspace, size_t workspace_bytes,
+                           cudaStream_t stream);
+
+typedef struct {
+  int32_t out_dtype;      /* race_dtype_t of the result                            */
+  int32_t b_square;       /* 1: b's scales are of 128 x 128 blocks, 0: of its rows  */
+  int64_t m, n, k;        /* a [m][k], b [n][k], result [m][n] = a b^T              */
+  int32_t wait_polls;     /* polls of each bounded device wait (0 = default, 2^22)  */
+  int32_t reserved;       /* 0                                                     */
+} race_matmul_desc_t;
+
+/* result = a b^T of 8-bit operands, every 128-long partial product scaled in
+ * 32 bits by both its scales and summed in 32 bits in a fixed order.  status:
+ * optional word in memory that the device can write (pinned host memory serves);
+ * RACE_DEV_* bits are set in it where a kernel gave up on a bounded wait. */
+int race_scaled_matmul(const race_matmul_desc_t* desc, race_blocks_t a, race_blocks_t b,
+                       race_rows_t result, uint32_t* status, void* workspace,
+                       size_t workspace_bytes, cudaStream_t stream);
+/* Workspace bytes of race_scaled_matmul (0 for most shapes). */
+size_t race_scaled_matmul_workspace(const race_matmul_desc_t* desc);
+
+/* One tensor of an optimizer step.  States in 8 bits: exp_avg and exp_avg_sq
+ * are codes (the second of the square root of the average), with one scale for
+ * each 128 consecutive elements in the *_scale arrays, both with room for numel
+ * rounded up to 128; states in 32 bits: float32, the *_scale pointers NULL. */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  int64_t numel;
+  uint64_t first;         /* index of element 0 in the noise of stochastic rounding */
+  int32_t dtype;          /* race_dtype_t of param and grad                        */
+  int32_t step;           /* steps taken before this one                           */
+} race_adamw_tensor_t;
+
+typedef struct {
+  double lr, beta_one, beta_two, eps, weight_decay;
+  uint32_t seed;
+  int32_t state_bits;     /* 8 or 32 */
+} race_adamw_desc_t;
+
+/* p -= lr * weight_decay * p; m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g^2;
+ * p -= lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps), t = step + 1, for every
+ * tensor of the list (a host array; it is passed to the kernels by value, so
+ * it may be freed on return).  bfloat16 parameters and 8-bit states are
+ * rounded up or down with the probability of the part cut off, by noise that
+ * is a function of seed, t and the element's index alone. */
+int race_adamw(const race_adamw_desc_t* desc, const race_adamw_tensor_t* tensors, int64_t count,
+               cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,6 +33,8 @@ SYMBOLS = (
     "race_last_kernels", "race_status_clear", "race_device_status",
     "race_comm_unique_id", "race_comm_init", "race_comm_destroy", "race_set_comm",
     "race_comm_error",
+    "race_quantize", "race_rms_norm", "race_rms_norm_workspace", "race_rms_norm_backward",
+    "race_scaled_matmul", "race_scaled_matmul_workspace", "race_adamw",
 )
 
 
@@ -58,6 +60,41 @@ class RaceSizes(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t), ("total_bytes", ctypes.c_size_t),
                 ("slot_floats", ctypes.c_int32), ("chunk", ctypes.c_int32),
                 ("num_chunks", ctypes.c_int64)]
+
+
+class RaceRows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("ld", ctypes.c_int64)]
+
+
+class RaceBlocks(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("ld", ctypes.c_int64), ("scales", ctypes.c_void_p),
+                ("stride_row", ctypes.c_int64), ("stride_block", ctypes.c_int64)]
+
+
+class RaceNormDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
+                ("rows", ctypes.c_int64), ("width", ctypes.c_int64), ("eps", ctypes.c_float)]
+
+
+class RaceMatmulDesc(ctypes.Structure):
+    _fields_ = [("out_dtype", ctypes.c_int32), ("b_square", ctypes.c_int32),
+                ("m", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64),
+                ("wait_polls", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class RaceAdamwTensor(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+                ("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
+                ("exp_avg_scale", ctypes.c_void_p), ("exp_avg_sq_scale", ctypes.c_void_p),
+                ("numel", ctypes.c_int64), ("first", ctypes.c_uint64),
+                ("dtype", ctypes.c_int32), ("step", ctypes.c_int32)]
+
+
+class RaceAdamwDesc(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta_one", ctypes.c_double),
+                ("beta_two", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("seed", ctypes.c_uint32),
+                ("state_bits", ctypes.c_int32)]
 
 
 class RaceError(RuntimeError):
@@ -109,6 +146,18 @@ _SIGS = {
     "race_probs_workspace": ([ctypes.POINTER(RaceDesc)], ctypes.c_size_t),
     "race_probs_backward": ([ctypes.POINTER(RaceDesc), _T, _P, _P, _P, _T, _P, ctypes.c_int, _P,
                              ctypes.c_size_t, _P], ctypes.c_int),
+    "race_quantize": ([RaceRows, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+                       RaceBlocks, RaceBlocks, _P], ctypes.c_int),
+    "race_rms_norm": ([ctypes.POINTER(RaceNormDesc), RaceRows, RaceRows, _P, RaceRows, RaceBlocks,
+                       RaceRows, _P, _P], ctypes.c_int),
+    "race_rms_norm_workspace": ([ctypes.POINTER(RaceNormDesc)], ctypes.c_size_t),
+    "race_rms_norm_backward": ([ctypes.POINTER(RaceNormDesc), RaceRows, RaceRows, RaceRows, _P, _P,
+                                RaceRows, _P, _P, ctypes.c_size_t, _P], ctypes.c_int),
+    "race_scaled_matmul": ([ctypes.POINTER(RaceMatmulDesc), RaceBlocks, RaceBlocks, RaceRows, _P,
+                            _P, ctypes.c_size_t, _P], ctypes.c_int),
+    "race_scaled_matmul_workspace": ([ctypes.POINTER(RaceMatmulDesc)], ctypes.c_size_t),
+    "race_adamw": ([ctypes.POINTER(RaceAdamwDesc), ctypes.POINTER(RaceAdamwTensor),
+                    ctypes.c_int64, _P], ctypes.c_int),
 }
 
 

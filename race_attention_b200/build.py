@@ -2,7 +2,7 @@
 
     python -m race_attention_b200.build      (or __graft_entry__.build())
 
-The three translation units compile in parallel; the result lands next to
+The translation units compile in parallel; the result lands next to
 this file so it travels with the source tree.
 """
 from __future__ import annotations
@@ -18,7 +18,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "librace_b200.so")
 SOURCES = ["race_capi.cu", "race_f32_d32.cu", "race_f32_d64.cu", "race_bf16_d32.cu",
-           "race_bf16_d64.cu", "race_probs.cu", "race_comm.cu"]
+           "race_bf16_d64.cu", "race_probs.cu", "race_comm.cu", "race_norm.cu", "race_quant.cu",
+           "race_matmul.cu", "race_adamw.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-I" + os.path.join(ROOT, "include"), "-I" + CSRC]

@@ -1,0 +1,300 @@
+// race_adamw.cu -- one AdamW step over many tensors in one launch, states in 32
+// or in 8 bits.
+//
+//   p -= lr wd p;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+//   p -= lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Nothing is used twice, so memory bounds the step: float32 with 32-bit states
+// moves 28 bytes a parameter, bfloat16 with 8-bit states 10.1.  The tensors'
+// addresses travel in the kernel's parameters (up to 384 tensors in the 32 KB
+// that a launch carries), so a step needs no copy to the device and can be
+// captured; a CTA finds its 2048 elements by bisection over the running chunk
+// counts.  A thread holds 8 consecutive elements, half a warp one 128-element
+// block of the states.
+//
+// 8-bit states.  m and sqrt(v) are held as e4m3 codes with one scale for each
+// 128 elements (the root halves v's range of exponents).  Codes are 6 to 12 %
+// apart while b2 = 0.999 moves sqrt(v) by at most 0.05 % of itself downwards a
+// step, so rounding to nearest would never let a state decay; the states are
+// rounded up or down with the probability of the part cut off instead, which is
+// right on average.  A second moment above zero is held as at least the
+// smallest code: as zero, it would leave eps alone in the denominator.
+// bfloat16 parameters (2^-9 of themselves apart) are rounded the same way.
+// The noise is a hash of the element's index, the seed and t, two odd
+// multipliers (2^32 over the golden ratio; the fraction of sqrt(2)) between shifts.
+#include <cmath>
+
+#include "race_api.h"
+#include "race_lowp.cuh"
+
+namespace race {
+namespace adamw {
+
+using namespace lowp;
+
+constexpr int NT = 256;
+constexpr int CHUNK = 8 * NT;
+constexpr uint32_t kGolden = 0x9E3779B1u, kRootTwo = 0x6A09E667u;
+
+struct Item {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  float* ms;
+  float* vs;
+  int64_t n;
+  uint32_t first;
+  uint32_t key;            // seed and step
+  float step_size;         // lr / (1 - b1^t)
+  float root_scale;        // 1 / sqrt(1 - b2^t)
+  int flags;               // 1: bf16, 2: vector access
+};
+
+template <int N>
+struct Args {
+  int count;
+  float keep;              // 1 - lr wd
+  float b1, c1, b2, c2, eps;
+  int32_t end[N];          // chunks up to and with tensor i
+  Item item[N];
+};
+
+__device__ __forceinline__ uint32_t noise(uint32_t i, uint32_t key) {
+  uint32_t h = (i ^ key) * kGolden;
+  h = (h ^ (h >> 15)) * kRootTwo;
+  return h ^ (h >> 16);
+}
+
+// y in [0, 448] up or down to the 8-bit format, r16 of 65536ths deciding: below
+// 2^-6 the format's steps are even, as they are for every number of the binade
+// that adding 2^-6 moves y to.
+__device__ __forceinline__ float dither(float y, uint32_t r16) {
+  const float low = y < 0.015625f ? 0.015625f : 0.f;
+  const uint32_t b = (__float_as_uint(y + low) + (r16 << 4)) & ~0xfffffu;
+  return __uint_as_float(b) - low;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_some(const T* p, bool vec, int n, float (&v)[8]) {
+  if (vec && n >= 8) {
+    load8(p, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void store_some(T* p, bool vec, int n, const float (&v)[8]) {
+  if (vec && n >= 8) {
+    store8(p, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) p[i] = from_f32<T>(v[i]);
+}
+
+// eight codes of a state's block (states start on 128-element boundaries, so
+// whole words are always inside them)
+__device__ __forceinline__ void load_codes(const void* p, int64_t at, float s, float (&v)[8]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p) + at);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = i < 2 ? u.x : u.y;
+    const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * (i & 1))), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hr));
+    v[2 * i] = f.x * s;
+    v[2 * i + 1] = f.y * s;
+  }
+}
+
+// Holds a state's eight values of this lane; `upper` picks the half of the noise.
+template <bool ROOT>
+__device__ __forceinline__ void hold(void* p, float* scales, int64_t at, bool live, const float (&x)[8],
+                                     const uint32_t (&r)[8], int lane) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = max(a, mag(x[i]));
+  const float s = scale_of(max_over(a, 16)), inv = 1.f / s;
+  if (!live) return;
+  float c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = fminf(fabsf(x[i]) * inv, kTop);
+    float d = dither(y, ROOT ? r[i] >> 16 : r[i] & 0xffffu);
+    if (ROOT && d == 0.f && y > 0.f) d = 0.001953125f;
+    c[i] = ROOT ? d : copysignf(d, x[i]);
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p) + at) = code8(c, 1.f);
+  if ((lane & 15) == 0) scales[at / kBlock] = s;
+}
+
+template <int N, bool EIGHT>
+__global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a) {
+  int lo = 0, hi = a.count - 1;
+  const int chunk = blockIdx.x;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (chunk < a.end[mid]) hi = mid; else lo = mid + 1;
+  }
+  const Item& it = a.item[lo];
+  const int64_t c0 = (int64_t)(chunk - (lo > 0 ? a.end[lo - 1] : 0)) * CHUNK;
+  const int lane = threadIdx.x & 31;
+  const int64_t at = c0 + 8 * (int64_t)threadIdx.x;
+  const int n = (int)min((int64_t)8, max((int64_t)0, it.n - at));    // elements of this thread
+  // a state's block is whole even where the tensor ends inside it
+  const bool live = at < ((it.n + kBlock - 1) & ~(int64_t)(kBlock - 1));
+  const bool vec = it.flags & 2, half = it.flags & 1;
+  float p[8], g[8], m[8], v[8];
+  if (half) {
+    load_some(static_cast<const bf16*>(it.p) + at, vec, n, p);
+    load_some(static_cast<const bf16*>(it.g) + at, vec, n, g);
+  } else {
+    load_some(static_cast<const float*>(it.p) + at, vec, n, p);
+    load_some(static_cast<const float*>(it.g) + at, vec, n, g);
+  }
+  if constexpr (EIGHT) {
+    if (live) {
+      load_codes(it.m, at, it.ms[at / kBlock], m);
+      load_codes(it.v, at, it.vs[at / kBlock], v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m[i] = v[i] = 0.f;
+    }
+  } else {
+    load_some(static_cast<const float*>(it.m) + at, true, n, m);
+    load_some(static_cast<const float*>(it.v) + at, true, n, v);
+  }
+  const uint32_t i0 = it.first + (uint32_t)at;
+  float root[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // each operation rounded on its own, so that a restatement in elementary
+    // 32-bit operations gives the same states, bit for bit
+    m[i] = __fadd_rn(__fmul_rn(a.b1, m[i]), __fmul_rn(a.c1, g[i]));
+    v[i] = __fadd_rn(__fmul_rn(a.b2, v[i]), __fmul_rn(__fmul_rn(a.c2, g[i]), g[i]));
+    root[i] = sqrtf(v[i]);
+    p[i] = fmaf(-it.step_size, m[i] / fmaf(root[i], it.root_scale, a.eps), p[i] * a.keep);
+  }
+  if (half) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t b = __float_as_uint(p[i]);
+      // infinities and NaN keep their bits
+      if ((b & 0x7f800000u) != 0x7f800000u)
+        p[i] = __uint_as_float((b + (noise(i0 + i, it.key + 1) & 0xffffu)) & ~0xffffu);
+    }
+    store_some(static_cast<bf16*>(it.p) + at, vec, n, p);
+  } else {
+    store_some(static_cast<float*>(it.p) + at, vec, n, p);
+  }
+  if constexpr (EIGHT) {
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      r[i] = noise(i0 + i, it.key);
+      if (i >= n) m[i] = root[i] = 0.f;      // past the tensor: held as zero
+    }
+    hold<false>(it.m, it.ms, at, live, m, r, lane);
+    hold<true>(it.v, it.vs, at, live, root, r, lane);
+  } else {
+    store_some(static_cast<float*>(it.m) + at, true, n, m);
+    store_some(static_cast<float*>(it.v) + at, true, n, v);
+  }
+}
+
+template <int N>
+int launch(const race_adamw_desc_t* d, const race_adamw_tensor_t* t, int count, cudaStream_t s) {
+  static_assert(sizeof(Args<N>) <= 32764, "a launch carries 32764 bytes of parameters");
+  Args<N> a;
+  a.keep = (float)(1.0 - d->lr * d->weight_decay);
+  a.b1 = (float)d->beta_one;
+  a.c1 = (float)(1.0 - d->beta_one);
+  a.b2 = (float)d->beta_two;
+  a.c2 = (float)(1.0 - d->beta_two);
+  a.eps = (float)d->eps;
+  int64_t chunks = 0;
+  int used = 0;
+  for (int i = 0; i < count; ++i) {
+    const race_adamw_tensor_t& x = t[i];
+    if (x.numel == 0) continue;
+    const int32_t step = x.step + 1;
+    Item& it = a.item[used];
+    const int es = x.dtype == RACE_BF16 ? 2 : 4;
+    it.p = x.param;
+    it.g = x.grad;
+    it.m = x.exp_avg;
+    it.v = x.exp_avg_sq;
+    it.ms = x.exp_avg_scale;
+    it.vs = x.exp_avg_sq_scale;
+    it.n = x.numel;
+    it.first = (uint32_t)x.first;
+    it.key = d->seed + kGolden * (uint32_t)step;
+    it.step_size = (float)(d->lr / (1.0 - std::pow(d->beta_one, step)));
+    it.root_scale = (float)(1.0 / std::sqrt(1.0 - std::pow(d->beta_two, step)));
+    const bool vec = reinterpret_cast<uintptr_t>(x.param) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(x.grad) % 16 == 0;
+    it.flags = (es == 2 ? 1 : 0) | (vec ? 2 : 0);
+    chunks += (x.numel + CHUNK - 1) / CHUNK;
+    if (chunks >= (int64_t(1) << 31)) {
+      api_note("adamw: 2^42 elements and more in one launch");
+      return RACE_ERR_UNSUPPORTED;
+    }
+    a.end[used++] = (int32_t)chunks;
+  }
+  a.count = used;
+  if (used == 0) return RACE_OK;
+  if (d->state_bits == 8)
+    k_adamw<N, true><<<(unsigned)chunks, NT, 0, s>>>(a);
+  else
+    k_adamw<N, false><<<(unsigned)chunks, NT, 0, s>>>(a);
+  api_log(d->state_bits == 8 ? "adamw_8bit" : "adamw");
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? RACE_OK : api_cuda_fail(e);
+}
+
+constexpr int kFew = 40, kMany = 360;
+
+}  // namespace adamw
+}  // namespace race
+
+using namespace race;
+
+extern "C" int race_adamw(const race_adamw_desc_t* desc, const race_adamw_tensor_t* tensors,
+                          int64_t count, cudaStream_t stream) {
+  ApiCall call;
+  if (desc == nullptr || count < 0 || (count > 0 && tensors == nullptr)) return RACE_ERR_INVALID;
+  if (desc->state_bits != 8 && desc->state_bits != 32) return RACE_ERR_INVALID;
+  if (!(desc->beta_one >= 0 && desc->beta_one < 1) || !(desc->beta_two >= 0 && desc->beta_two < 1) ||
+      !(desc->eps >= 0))
+    return RACE_ERR_INVALID;
+  for (int64_t i = 0; i < count; ++i) {
+    const race_adamw_tensor_t& t = tensors[i];
+    if (t.numel < 0 || t.step < 0 || (t.dtype != RACE_F32 && t.dtype != RACE_BF16)) return RACE_ERR_INVALID;
+    if (t.numel == 0) continue;
+    if (t.param == nullptr || t.grad == nullptr || t.exp_avg == nullptr || t.exp_avg_sq == nullptr)
+      return RACE_ERR_INVALID;
+    if (desc->state_bits == 8 && (t.exp_avg_scale == nullptr || t.exp_avg_sq_scale == nullptr))
+      return RACE_ERR_INVALID;
+    const int es = t.dtype == RACE_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(t.param) % es != 0 || reinterpret_cast<uintptr_t>(t.grad) % es != 0 ||
+        reinterpret_cast<uintptr_t>(t.exp_avg) % 16 != 0 || reinterpret_cast<uintptr_t>(t.exp_avg_sq) % 16 != 0)
+      return RACE_ERR_ALIGN;
+  }
+  if (count == 0) return RACE_OK;
+  RACE_CALL(api_bind(stream));
+  for (int64_t i = 0; i < count;) {
+    const int64_t left = count - i;
+    if (left <= adamw::kFew) {
+      RACE_CALL(adamw::launch<adamw::kFew>(desc, tensors + i, (int)left, stream));
+      break;
+    }
+    const int now = (int)(left < adamw::kMany ? left : adamw::kMany);
+    RACE_CALL(adamw::launch<adamw::kMany>(desc, tensors + i, now, stream));
+    i += now;
+  }
+  return RACE_OK;
+}

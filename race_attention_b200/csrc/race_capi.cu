@@ -5,6 +5,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "race_api.h"
 #include "race_b200.h"
 #include "race_launch.h"
 
@@ -32,20 +33,22 @@ thread_local cudaStream_t g_bound_stream = nullptr;
 
 // Clears the calling thread's log when the outermost entry point of a call
 // starts and publishes it when that entry point returns.
+void new_scope() {
+  if (g_api_depth++ == 0) {
+    g_kernels[0] = '\0';
+    g_cuda_err[0] = '\0';
+    g_bound_valid = false;
+  }
+}
+void end_scope() {
+  if (--g_api_depth == 0) {
+    std::lock_guard<std::mutex> lock(g_log_mu);
+    std::memcpy(g_kernels_last, g_kernels, sizeof(g_kernels));
+  }
+}
 struct ApiScope {
-  ApiScope() {
-    if (g_api_depth++ == 0) {
-      g_kernels[0] = '\0';
-      g_cuda_err[0] = '\0';
-      g_bound_valid = false;
-    }
-  }
-  ~ApiScope() {
-    if (--g_api_depth == 0) {
-      std::lock_guard<std::mutex> lock(g_log_mu);
-      std::memcpy(g_kernels_last, g_kernels, sizeof(g_kernels));
-    }
-  }
+  ApiScope() { new_scope(); }
+  ~ApiScope() { end_scope(); }
 };
 
 void log_kernel(const char* name, const char* note = nullptr) {
@@ -571,6 +574,47 @@ bool encode_map3(CUtensorMap* m, const float* base, int64_t N, int64_t T, int C,
   }
   return true;
 }
+
+}  // namespace
+
+void api_begin() { new_scope(); }
+void api_end() { end_scope(); }
+int api_bind(cudaStream_t stream) {
+  // A stream's device cannot be asked for while it is being captured; the
+  // capturing thread has its context current.
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(stream, &st);
+  if (e != cudaSuccess) return cuda_fail(e);
+  return st == cudaStreamCaptureStatusNone ? bind_device(stream) : RACE_OK;
+}
+int api_cuda_fail(cudaError_t e) { return cuda_fail(e); }
+void api_log(const char* kernel) { log_kernel(kernel); }
+int api_sm_count() { return sm_count(); }
+void api_note(const char* text) { std::snprintf(g_cuda_err, sizeof(g_cuda_err), "%s", text); }
+
+bool api_encode_bytes(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld,
+                      int box_rows) {
+  const EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) {
+    api_note("cuTensorMapEncodeTiled not found");
+    return false;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides,
+                        box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    std::snprintf(g_cuda_err, sizeof(g_cuda_err), "tensor map: encode error %d (%lld x %lld, ld %lld)",
+                  (int)r, (long long)rows, (long long)cols, (long long)ld);
+    return false;
+  }
+  return true;
+}
+
+namespace {
 
 const char* kernel_name(KernelId id) {
   switch (id) {

@@ -1,0 +1,452 @@
+// race_norm.cu -- root-mean-square norm with the residual's addition, its
+// backward pass, and its form with 8-bit results.
+//
+//   h = x + residual;  r = 1 / sqrt(mean(h^2) + eps);  y = h r w
+//   g = dy w;  dx = dh + r (g - h r^2 mean(g h));  dw = sum over rows of dy h r
+//
+// Both passes are bound by memory: forward 3 rows moved (x, residual, h) and
+// one written (y, or a quarter to a half of it in 8 bits), backward 3 read and one
+// written.  So a row is read once and held in registers between its sum and its
+// use: a warp holds up to 1024 columns (32 values a lane), wider rows are
+// spread over 4, 16 or 32 warps of one CTA.  Columns come in spans of 256 for each warp,
+// two 8-bit blocks, so a block's maximum never leaves its warp: with vector
+// loads a lane holds 8 consecutive columns and half a warp holds a block,
+// otherwise (odd widths or strides) lane l holds columns l, l + 32, ... and the
+// whole warp holds a block in four of its eight values.
+#include "race_api.h"
+#include "race_lowp.cuh"
+
+namespace race {
+namespace norm {
+
+using namespace lowp;
+
+struct FwdArgs {
+  const void* x; int64_t ldx;
+  const void* res; int64_t ldr;
+  const void* w; int wbf16;
+  void* y; int64_t ldy;
+  void* h; int64_t ldh;
+  uint8_t* codes; int64_t ldc;
+  float* scales; int64_t sr, sb;
+  float* rstd;
+  int64_t rows; int width;
+  float eps;
+};
+
+struct BwdArgs {
+  const void* dy; int64_t lddy;
+  const void* dh; int64_t lddh;
+  const void* h; int64_t ldh;
+  const void* w; int wbf16;
+  const float* rstd;
+  void* dx; int64_t lddx;
+  float* part;            // [CTAs][width]
+  int64_t rows; int width;
+};
+
+// column of value i of span s
+template <bool VEC>
+__device__ __forceinline__ int col_of(int s, int lane, int i) {
+  return 256 * s + (VEC ? 8 * lane + i : 32 * i + lane);
+}
+
+// Vector loads need every row's base on 16 bytes; the last vector of a row may
+// be partial (width % 8), its columns then come one by one.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_span(const T* row, int s, int lane, int width, float (&v)[8]) {
+  if constexpr (VEC) {
+    const int c = 256 * s + 8 * lane;
+    if (c + 8 <= width) {
+      load8(row + c, v);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = col_of<VEC>(s, lane, i);
+    v[i] = c < width ? to_f32(row[c]) : 0.f;
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_span(T* row, int s, int lane, int width, const float (&v)[8]) {
+  if constexpr (VEC) {
+    const int c = 256 * s + 8 * lane;
+    if (c + 8 <= width) {
+      store8(row + c, v);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = col_of<VEC>(s, lane, i);
+    if (c < width) row[c] = from_f32<T>(v[i]);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void load_weight(const void* w, int wbf16, int s, int lane, int width,
+                                            float (&v)[8]) {
+  if (wbf16)
+    load_span<bf16, VEC>(static_cast<const bf16*>(w), s, lane, width, v);
+  else
+    load_span<float, VEC>(static_cast<const float*>(w), s, lane, width, v);
+}
+
+__device__ __forceinline__ float warp_sum(float a) {
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  return a;
+}
+
+// Sum over the WPR warps of a row, in the order of the warps.  `slot` alternates
+// between calls, so that one barrier serves each.
+template <int WPR>
+__device__ __forceinline__ float row_sum(float a, float (*slot)[32], int which) {
+  a = warp_sum(a);
+  if constexpr (WPR > 1) {
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) slot[which][warp] = a;
+    __syncthreads();
+    a = 0.f;
+#pragma unroll
+    for (int i = 0; i < WPR; ++i) a += slot[which][i];
+  }
+  return a;
+}
+
+constexpr int threads_of(int wpr) { return wpr == 1 ? 128 : 32 * wpr; }
+
+template <typename T, bool VEC, int V, int WPR, bool Q>
+__global__ void __launch_bounds__(threads_of(WPR)) k_rms_fwd(const FwdArgs a) {
+  __shared__ float slot[2][32];
+  constexpr int RPC = threads_of(WPR) / (32 * WPR);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * RPC + warp / WPR;
+  const int w0 = warp % WPR;
+  if (row >= a.rows) return;                 // whole warps only; WPR > 1 has one row per CTA
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  float h[V][8];
+#pragma unroll
+  for (int j = 0; j < V; ++j) load_span<T, VEC>(x, j * WPR + w0, lane, a.width, h[j]);
+  if (a.res != nullptr) {
+    const T* r = static_cast<const T*>(a.res) + row * a.ldr;
+    float t[V][8];
+#pragma unroll
+    for (int j = 0; j < V; ++j) load_span<T, VEC>(r, j * WPR + w0, lane, a.width, t[j]);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[j][i] += t[j][i];
+    T* o = static_cast<T*>(a.h) + row * a.ldh;
+#pragma unroll
+    for (int j = 0; j < V; ++j) store_span<T, VEC>(o, j * WPR + w0, lane, a.width, h[j]);
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
+  ss = row_sum<WPR>(ss, slot, 0);
+  const float rs = 1.f / sqrtf(ss / (float)a.width + a.eps);
+  if (a.rstd != nullptr && lane == 0 && w0 == 0) a.rstd[row] = rs;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int s = j * WPR + w0;
+    if (256 * s >= a.width) break;           // the same for the whole warp
+    float w[8];
+    load_weight<VEC>(a.w, a.wbf16, s, lane, a.width, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[j][i] = h[j][i] * rs * w[i];
+    if constexpr (!Q) {
+      store_span<T, VEC>(static_cast<T*>(a.y) + row * a.ldy, s, lane, a.width, h[j]);
+    } else {
+      uint8_t* c = a.codes + row * a.ldc;
+      float* sc = a.scales + row * a.sr;
+      if constexpr (VEC) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, mag(h[j][i]));
+        const float sv = scale_of(max_over(m, 16));
+        const int c0 = 256 * s + 8 * lane;
+        if (c0 < a.width) {                  // columns past the width hold zeros
+          *reinterpret_cast<uint2*>(c + c0) = code8(h[j], 1.f / sv);
+          if ((lane & 15) == 0) sc[(2 * s + (lane >> 4)) * a.sb] = sv;
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          uint32_t m = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m = max(m, mag(h[j][4 * b + i]));
+          const float sv = scale_of(max_over(m, 32));
+          const float inv = 1.f / sv;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int cc = col_of<false>(s, lane, 4 * b + i);
+            // the row's pitch is a multiple of 16: the rest of its last 16 bytes is zeroed
+            if (cc < ((a.width + 15) & ~15))
+              c[cc] = (uint8_t)code2(h[j][4 * b + i] * inv, 0.f);
+          }
+          if (lane == 0 && 256 * s + 128 * b < a.width) sc[(2 * s + b) * a.sb] = sv;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, bool VEC, int V, int WPR>
+__global__ void __launch_bounds__(threads_of(WPR)) k_rms_bwd(const BwdArgs a) {
+  __shared__ float slot[2][32];
+  constexpr int RPC = threads_of(WPR) / (32 * WPR);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int w0 = warp % WPR;
+  const int64_t step = (int64_t)gridDim.x * RPC;
+  float dw[V][8];
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[j][i] = 0.f;
+  int which = 0;
+  for (int64_t row = (int64_t)blockIdx.x * RPC + warp / WPR; row < a.rows; row += step) {
+    const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
+    const T* hr = static_cast<const T*>(a.h) + row * a.ldh;
+    const float rs = a.rstd[row];
+    float g[V][8], h[V][8];
+    float dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) load_span<T, VEC>(dy, j * WPR + w0, lane, a.width, g[j]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) load_span<T, VEC>(hr, j * WPR + w0, lane, a.width, h[j]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float w[8];
+      load_weight<VEC>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dw[j][i] = fmaf(g[j][i], h[j][i] * rs, dw[j][i]);
+        g[j][i] *= w[i];
+        dot = fmaf(g[j][i], h[j][i], dot);
+      }
+    }
+    dot = row_sum<WPR>(dot, slot, which);
+    which ^= 1;
+    const float c = dot / (float)a.width * rs * rs;
+    T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[j][i] = rs * (g[j][i] - h[j][i] * c);
+      if (a.dh != nullptr) {
+        float t[8];
+        load_span<T, VEC>(static_cast<const T*>(a.dh) + row * a.lddh, j * WPR + w0, lane, a.width, t);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[j][i] += t[i];
+      }
+      store_span<T, VEC>(dx, j * WPR + w0, lane, a.width, g[j]);
+    }
+  }
+  float* part = a.part + (int64_t)blockIdx.x * a.width;
+  if constexpr (RPC == 1) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = col_of<VEC>(j * WPR + w0, lane, i);
+        if (c < a.width) part[c] = dw[j][i];
+      }
+  } else {
+    // the CTA's warps hold the same columns of different rows
+    __shared__ float red[RPC][256];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) red[warp][col_of<VEC>(0, lane, i)] = dw[j][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < 256; c += 32 * RPC) {
+        float t = 0.f;
+#pragma unroll
+        for (int r = 0; r < RPC; ++r) t += red[r][c];
+        if (256 * j + c < a.width) part[256 * j + c] = t;
+      }
+    }
+  }
+}
+
+// dweight[c] = sum over the CTAs' partial rows, in their order within 8 strands
+__global__ void __launch_bounds__(256) k_rms_dweight(const float* __restrict__ part, int parts,
+                                                     int width, void* __restrict__ dw, int wbf16) {
+  __shared__ float red[8][33];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5;
+  float t = 0.f;
+  if (c < width)
+    for (int p = strand; p < parts; p += 8) t += part[(int64_t)p * width + c];
+  red[strand][threadIdx.x & 31] = t;
+  __syncthreads();
+  if (strand == 0 && c < width) {
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += red[i][threadIdx.x & 31];
+    if (wbf16)
+      static_cast<bf16*>(dw)[c] = from_f32<bf16>(t);
+    else
+      static_cast<float*>(dw)[c] = t;
+  }
+}
+
+// CTAs of the backward pass: enough to fill the SMs, no more than there are rows
+int bwd_ctas(const race_norm_desc_t* d, int wpr) {
+  const int rpc = threads_of(wpr) / (32 * wpr);
+  const int64_t most = (d->rows + rpc - 1) / rpc;
+  const int64_t fill = (int64_t)api_sm_count() * (wpr == 1 ? 8 : wpr == 4 ? 8 : wpr == 16 ? 2 : 1);
+  return (int)(most < fill ? most : fill);
+}
+
+int warps_per_row(int64_t width) {
+  return width <= 1024 ? 1 : width <= 4096 ? 4 : width <= 16384 ? 16 : 32;
+}
+
+template <typename T, bool VEC, int V, int WPR>
+void launch_fwd(const FwdArgs& a, cudaStream_t s) {
+  constexpr int RPC = threads_of(WPR) / (32 * WPR);
+  const unsigned grid = (unsigned)((a.rows + RPC - 1) / RPC);
+  if (a.codes != nullptr)
+    k_rms_fwd<T, VEC, V, WPR, true><<<grid, threads_of(WPR), 0, s>>>(a);
+  else
+    k_rms_fwd<T, VEC, V, WPR, false><<<grid, threads_of(WPR), 0, s>>>(a);
+}
+template <typename T, bool VEC, int V, int WPR>
+void launch_bwd(const BwdArgs& a, int grid, cudaStream_t s) {
+  k_rms_bwd<T, VEC, V, WPR><<<grid, threads_of(WPR), 0, s>>>(a);
+}
+
+// The spans a warp holds (V) follow from the width; the unvectorised form and
+// the widest rows are built once.
+template <typename F>
+void pick(bool f32, bool vec, int wpr, int v, F&& f) {
+#define RACE_PICK(V, W)                                                     \
+  if (wpr == W && (vec || V == (W == 32 ? 8 : 4)) && v <= V) {              \
+    if (vec) return f32 ? f(float(), std::true_type(), std::integral_constant<int, V>(), std::integral_constant<int, W>())  \
+                        : f(bf16(), std::true_type(), std::integral_constant<int, V>(), std::integral_constant<int, W>());  \
+    if constexpr (V == (W == 32 ? 8 : 4))                                   \
+      return f32 ? f(float(), std::false_type(), std::integral_constant<int, V>(), std::integral_constant<int, W>())        \
+                 : f(bf16(), std::false_type(), std::integral_constant<int, V>(), std::integral_constant<int, W>());        \
+  }
+  RACE_PICK(1, 1) RACE_PICK(2, 1) RACE_PICK(3, 1) RACE_PICK(4, 1)
+  RACE_PICK(2, 4) RACE_PICK(3, 4) RACE_PICK(4, 4)
+  RACE_PICK(2, 16) RACE_PICK(3, 16) RACE_PICK(4, 16)
+  RACE_PICK(8, 32)
+#undef RACE_PICK
+}
+
+bool aligned16(const void* p, int64_t ld, int es) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0;
+}
+
+int check_desc(const race_norm_desc_t* d) {
+  if (d == nullptr || d->rows < 0 || d->width < 1) return RACE_ERR_INVALID;
+  if (d->dtype != RACE_F32 && d->dtype != RACE_BF16) return RACE_ERR_INVALID;
+  if (d->weight_dtype != RACE_F32 && d->weight_dtype != RACE_BF16) return RACE_ERR_INVALID;
+  if (d->width > 65536 || d->rows >= (int64_t(1) << 31)) {
+    api_note("norm: width above 65536 or 2^31 rows and more");
+    return RACE_ERR_UNSUPPORTED;
+  }
+  return RACE_OK;
+}
+
+int check_rows(const race_norm_desc_t* d, race_rows_t r, bool wanted) {
+  if (r.data == nullptr) return wanted ? RACE_ERR_INVALID : RACE_OK;
+  if (reinterpret_cast<uintptr_t>(r.data) % (d->dtype == RACE_F32 ? 4 : 2) != 0) return RACE_ERR_ALIGN;
+  return d->rows <= 1 || r.ld >= d->width || r.ld == 0 ? RACE_OK : RACE_ERR_INVALID;
+}
+
+}  // namespace norm
+}  // namespace race
+
+using namespace race;
+
+extern "C" int race_rms_norm(const race_norm_desc_t* desc, race_rows_t x, race_rows_t residual,
+                             const void* weight, race_rows_t y, race_blocks_t y8, race_rows_t h,
+                             float* rstd, cudaStream_t stream) {
+  ApiCall call;
+  RACE_CALL(norm::check_desc(desc));
+  if (desc->rows == 0) return RACE_OK;
+  if (weight == nullptr || (y.data == nullptr) == (y8.codes == nullptr)) return RACE_ERR_INVALID;
+  RACE_CALL(norm::check_rows(desc, x, true));
+  RACE_CALL(norm::check_rows(desc, residual, false));
+  RACE_CALL(norm::check_rows(desc, y, false));
+  RACE_CALL(norm::check_rows(desc, h, residual.data != nullptr));
+  if ((y.data != nullptr && y.ld < desc->width && desc->rows > 1) ||
+      (residual.data != nullptr && h.ld < desc->width && desc->rows > 1))
+    return RACE_ERR_INVALID;                 // results may not overlap
+  if (y8.codes != nullptr) {
+    if (y8.scales == nullptr) return RACE_ERR_INVALID;
+    if (reinterpret_cast<uintptr_t>(y8.codes) % 16 != 0 || y8.ld % 16 != 0) return RACE_ERR_ALIGN;
+    if (y8.ld < desc->width) return RACE_ERR_INVALID;
+  }
+  RACE_CALL(api_bind(stream));
+  norm::FwdArgs a{x.data, x.ld, residual.data, residual.ld, weight, desc->weight_dtype == RACE_BF16,
+                  y.data, y.ld, h.data, h.ld, static_cast<uint8_t*>(y8.codes), y8.ld, y8.scales,
+                  y8.stride_row, y8.stride_block, rstd, desc->rows, (int)desc->width, desc->eps};
+  const bool f32 = desc->dtype == RACE_F32;
+  const int es = f32 ? 4 : 2;
+  const bool vec = norm::aligned16(x.data, x.ld, es) && norm::aligned16(weight, 0, 1) &&
+                   (residual.data == nullptr || (norm::aligned16(residual.data, residual.ld, es) &&
+                                                 norm::aligned16(h.data, h.ld, es))) &&
+                   (y.data == nullptr || norm::aligned16(y.data, y.ld, es));
+  const int wpr = norm::warps_per_row(desc->width);
+  const int v = (int)((desc->width + 256 * wpr - 1) / (256 * wpr));
+  norm::pick(f32, vec, wpr, v, [&](auto t, auto ve, auto vv, auto ww) {
+    norm::launch_fwd<decltype(t), decltype(ve)::value, decltype(vv)::value, decltype(ww)::value>(a, stream);
+  });
+  api_log(y8.codes != nullptr ? "rms_fwd_8bit" : "rms_fwd");
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? RACE_OK : api_cuda_fail(e);
+}
+
+extern "C" size_t race_rms_norm_workspace(const race_norm_desc_t* desc) {
+  if (norm::check_desc(desc) != RACE_OK) return 0;
+  const int ctas = norm::bwd_ctas(desc, norm::warps_per_row(desc->width));
+  return (size_t)(ctas > 0 ? ctas : 1) * (size_t)desc->width * sizeof(float);
+}
+
+extern "C" int race_rms_norm_backward(const race_norm_desc_t* desc, race_rows_t dy, race_rows_t dh,
+                                      race_rows_t h, const void* weight, const float* rstd,
+                                      race_rows_t dx, void* dweight, void* workspace,
+                                      size_t workspace_bytes, cudaStream_t stream) {
+  ApiCall call;
+  RACE_CALL(norm::check_desc(desc));
+  const bool any = desc->rows > 0;
+  if (weight == nullptr || dweight == nullptr || (any && rstd == nullptr)) return RACE_ERR_INVALID;
+  RACE_CALL(norm::check_rows(desc, dy, any));
+  RACE_CALL(norm::check_rows(desc, dh, false));
+  RACE_CALL(norm::check_rows(desc, h, any));
+  RACE_CALL(norm::check_rows(desc, dx, any));
+  if (desc->rows > 1 && dx.ld < desc->width) return RACE_ERR_INVALID;
+  RACE_CALL(api_bind(stream));
+  const int wb = desc->weight_dtype == RACE_BF16;
+  if (!any) {
+    const cudaError_t e = cudaMemsetAsync(dweight, 0, (size_t)desc->width * (wb ? 2 : 4), stream);
+    return e == cudaSuccess ? RACE_OK : api_cuda_fail(e);
+  }
+  if (workspace == nullptr || workspace_bytes < race_rms_norm_workspace(desc)) return RACE_ERR_WORKSPACE;
+  norm::BwdArgs a{dy.data, dy.ld, dh.data, dh.ld, h.data, h.ld, weight, wb, rstd, dx.data, dx.ld,
+                  static_cast<float*>(workspace), desc->rows, (int)desc->width};
+  const bool f32 = desc->dtype == RACE_F32;
+  const int es = f32 ? 4 : 2;
+  const bool vec = norm::aligned16(dy.data, dy.ld, es) && norm::aligned16(h.data, h.ld, es) &&
+                   norm::aligned16(dx.data, dx.ld, es) && norm::aligned16(weight, 0, 1) &&
+                   (dh.data == nullptr || norm::aligned16(dh.data, dh.ld, es));
+  const int wpr = norm::warps_per_row(desc->width);
+  const int v = (int)((desc->width + 256 * wpr - 1) / (256 * wpr));
+  const int grid = norm::bwd_ctas(desc, wpr);
+  norm::pick(f32, vec, wpr, v, [&](auto t, auto ve, auto vv, auto ww) {
+    norm::launch_bwd<decltype(t), decltype(ve)::value, decltype(vv)::value, decltype(ww)::value>(a, grid, stream);
+  });
+  api_log("rms_bwd");
+  norm::k_rms_dweight<<<(unsigned)((desc->width + 31) / 32), 256, 0, stream>>>(
+      a.part, grid, a.width, dweight, wb);
+  api_log("rms_dweight");
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? RACE_OK : api_cuda_fail(e);
+}

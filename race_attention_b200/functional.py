@@ -15,6 +15,7 @@ save the inputs and eps, call the kernel forward / backward) is played by
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional
 
@@ -111,10 +112,46 @@ class DeviceStatus:
 device_status = DeviceStatus()
 
 
+class HostStatus:
+    """Status word of the 8-bit products, one for each device, in pinned host
+    memory that the kernels write only when they give up on a bounded wait: a
+    call looks at it without a copy or a synchronisation and reports what
+    earlier calls left there."""
+
+    def __init__(self):
+        self.words = {}
+
+    def word(self, device: torch.device):
+        """(address, host view) of the device's word."""
+        entry = self.words.get(device.index)
+        if entry is None:
+            host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+            entry = (host.data_ptr(), ctypes.c_uint32.from_address(host.data_ptr()), host)
+            self.words[device.index] = entry
+        if entry[1].value:
+            self.fail(entry)
+        return entry[0]
+
+    def fail(self, entry) -> None:
+        word, entry[1].value = entry[1].value, 0
+        raise _lib.RaceError(f"race_b200 device status 0x{word:x}: a kernel gave up on a bounded "
+                             "wait (timeout); the outputs of that call are incomplete")
+
+    def check(self) -> None:
+        for index, entry in list(self.words.items()):
+            torch.cuda.synchronize(index)
+            if entry[1].value:
+                self.fail(entry)
+
+
+host_status = HostStatus()
+
+
 def check_device_status() -> None:
     """Waits for the outstanding status reads and raises RaceError if any
     forward or backward since the last check ended a kernel early."""
     device_status.check(wait=True)
+    host_status.check()
 
 
 _NORMS = {"bucket": _lib.RACE_NORM_BUCKET, "global": _lib.RACE_NORM_GLOBAL}

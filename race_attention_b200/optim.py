@@ -1,0 +1,216 @@
+"""AdamW over all tensors of a model in one launch, with states in 32 or 8 bits.
+
+The reference trains with torch.optim.AdamW; this optimizer has its update rule
+and its arguments.  States live in one allocation each for all parameters,
+every tensor starting on a multiple of 128 elements.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import RaceAdamwDesc, RaceAdamwTensor, check
+from .fp8 import BLOCK, F8, _on, _raw_stream
+from .functional import _SUPPORTED
+
+
+class AdamW(torch.optim.Optimizer):
+    """p -= lr wd p; m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g^2;
+    p -= lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).
+
+    params: float32 or bfloat16 CUDA tensors of one device, contiguous, with
+      gradients of their own type; parameter groups may set lr, betas, eps and
+      weight_decay.  A parameter without a gradient is left alone.
+    state_bits: 32, or 8: m and the square root of v as e4m3 codes with a
+      float32 scale for each 128 elements (2.06 bytes a parameter in place of
+      8).  8-bit states and bfloat16 parameters are rounded up or down with the
+      probability of the part cut off, so that changes smaller than a step of
+      the format are not lost; a second moment above zero is never held as zero.
+    seed: of that rounding; equal seeds and equal inputs give equal results.
+
+    ``exp_avg``, ``exp_avg_sq`` and, with 8 bits, ``exp_avg_scale`` and
+    ``exp_avg_sq_scale`` are the states of all parameters (``offsets`` says
+    where each begins); with 8 bits ``exp_avg_sq`` holds the codes of sqrt(v)."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, state_bits: int = 32, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        self._check_group({"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay})
+        self.state_bits = state_bits
+        self.seed = int(seed) & 0xFFFFFFFF
+        self.offsets, self._sizes = {}, {}
+        self._total = 0
+        self._tables = {}
+        self.exp_avg = self.exp_avg_sq = None
+        self.exp_avg_scale = self.exp_avg_sq_scale = None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    @staticmethod
+    def _check_group(g) -> None:
+        if not g["lr"] >= 0 or not g["eps"] >= 0 or not g["weight_decay"] >= 0:
+            raise ValueError("lr, eps and weight_decay must not be negative")
+        if len(g["betas"]) != 2 or not all(0 <= b < 1 for b in g["betas"]):
+            raise ValueError("betas must be two numbers in [0, 1)")
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            self._check_group(group)
+            for p in group["params"]:
+                if not p.is_cuda:
+                    raise ValueError("AdamW runs on CUDA parameters only (no CPU fallback)")
+                if p.dtype not in _SUPPORTED:
+                    raise ValueError("parameters must be float32 or bfloat16")
+                if not p.is_contiguous():
+                    raise ValueError("parameters must be contiguous")
+                if p.device != self._device(group):
+                    raise ValueError("all parameters must be on one device")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+        before = self._total
+        for p in group["params"]:
+            self.offsets[p] = self._total
+            self._sizes[p] = p.numel()
+            self._total += -(-p.numel() // BLOCK) * BLOCK
+            self.state[p]["step"] = 0
+        self._grow(self._total - before)
+        self._tables.clear()
+
+    def _device(self, group) -> torch.device:
+        for g in self.param_groups:
+            for p in g["params"]:
+                return p.device
+        return group["params"][0].device
+
+    def _grow(self, n: int) -> None:
+        dev = self._device(self.param_groups[0])
+        dtype = torch.float32 if self.state_bits == 32 else F8
+        new = {"exp_avg": torch.zeros(n, dtype=dtype, device=dev),
+               "exp_avg_sq": torch.zeros(n, dtype=dtype, device=dev)}
+        if self.state_bits == 8:
+            new["exp_avg_scale"] = torch.zeros(n // BLOCK, dtype=torch.float32, device=dev)
+            new["exp_avg_sq_scale"] = torch.zeros(n // BLOCK, dtype=torch.float32, device=dev)
+        for name, t in new.items():
+            old = getattr(self, name)
+            if old is not None:
+                b = old.view(torch.uint8) if old.dtype == F8 else old
+                t = torch.cat((b, t.view(b.dtype))).view(dtype if old.dtype == F8 else old.dtype)
+            setattr(self, name, t)
+
+    def set_state(self, step: int, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor,
+                  exp_avg_scale: Optional[torch.Tensor] = None,
+                  exp_avg_sq_scale: Optional[torch.Tensor] = None) -> None:
+        """Takes over states of every parameter (in the layout of ``exp_avg``
+        and the others, whose memory is kept and written) after ``step`` steps."""
+        for name, t in (("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq),
+                        ("exp_avg_scale", exp_avg_scale), ("exp_avg_sq_scale", exp_avg_sq_scale)):
+            have = getattr(self, name)
+            if have is None and t is None:
+                continue
+            if (have is None or t is None or t.shape != have.shape or t.dtype != have.dtype
+                    or t.device != have.device or not t.is_contiguous()
+                    or t.data_ptr() % 16 != 0):
+                raise ValueError(f"{name} must be a contiguous tensor like this optimizer's own")
+        self.exp_avg, self.exp_avg_sq = exp_avg, exp_avg_sq
+        self.exp_avg_scale, self.exp_avg_sq_scale = exp_avg_scale, exp_avg_sq_scale
+        for s in self.state.values():
+            s["step"] = int(step)
+        self._tables.clear()
+
+    def state_dict(self):
+        groups, index = [], {}
+        for g in self.param_groups:
+            for p in g["params"]:
+                index[p] = len(index)
+            groups.append({**{k: v for k, v in g.items() if k != "params"},
+                           "params": [index[p] for p in g["params"]]})
+        return {"state": {index[p]: {"step": self.state[p]["step"], "first": self.offsets[p]} for p in index},
+                "param_groups": groups, "state_bits": self.state_bits, "seed": self.seed,
+                "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq,
+                "exp_avg_scale": self.exp_avg_scale, "exp_avg_sq_scale": self.exp_avg_sq_scale}
+
+    def load_state_dict(self, state_dict) -> None:
+        if state_dict["state_bits"] != self.state_bits:
+            raise ValueError(f"the states were kept in {state_dict['state_bits']} bits, this "
+                             f"optimizer has {self.state_bits}")
+        groups = state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("the parameter groups differ from this optimizer's")
+        params = [p for g in self.param_groups for p in g["params"]]
+        order = [i for g in groups for i in g["params"]]
+        if any(state_dict["state"][i]["first"] != self.offsets[p] for i, p in zip(order, params)):
+            raise ValueError("the parameters' sizes differ from this optimizer's")
+        dev = self.exp_avg.device
+        names = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+        self.set_state(0, *(None if state_dict[n] is None else state_dict[n].to(dev, copy=True)
+                            for n in names))
+        for i, p in zip(order, params):
+            self.state[p]["step"] = int(state_dict["state"][i]["step"])
+        for g, s in zip(self.param_groups, groups):
+            g.update({k: v for k, v in s.items() if k != "params"})
+        self.seed = int(state_dict["seed"]) & 0xFFFFFFFF
+
+    def _table(self, gi: int, params):
+        """The C array of a group's tensors, its constant fields filled in."""
+        t = self._tables.get(gi)
+        if t is None:
+            t = (RaceAdamwTensor * len(params))()
+            m, v = self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr()
+            size = self.exp_avg.element_size()
+            for e, p in zip(t, params):
+                at = self.offsets[p]
+                e.exp_avg, e.exp_avg_sq = m + at * size, v + at * size
+                if self.state_bits == 8:
+                    e.exp_avg_scale = self.exp_avg_scale.data_ptr() + at // BLOCK * 4
+                    e.exp_avg_sq_scale = self.exp_avg_sq_scale.data_ptr() + at // BLOCK * 4
+                e.first = at
+            self._tables[gi] = t
+        return t
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        lib = _lib.load()
+        dev = self.exp_avg.device
+        for gi, group in enumerate(self.param_groups):
+            params = group["params"]
+            table = self._table(gi, params)
+            kept, live = [], []       # gradients copied for this step, tensors that move
+            for e, p in zip(table, params):
+                g = p.grad
+                if g is None:
+                    e.numel = 0
+                    continue
+                if g.dtype != p.dtype or g.is_sparse or g.device != p.device:
+                    raise ValueError("gradients must be dense, on their parameter's device and of its type")
+                n = p.numel()
+                if not p.is_contiguous() or n != self._sizes[p] or p.device != dev \
+                        or p.dtype not in _SUPPORTED:
+                    raise ValueError("a parameter changed its size, layout, type or device since "
+                                     "the optimizer was built")
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    kept.append(g)
+                st = self.state[p]
+                e.param, e.grad, e.numel = p.data_ptr(), g.data_ptr(), n
+                e.dtype = _lib.RACE_F32 if p.dtype == torch.float32 else _lib.RACE_BF16
+                e.step = st["step"]
+                live.append(st)
+            if not live:
+                continue
+            b1, b2 = group["betas"]
+            desc = RaceAdamwDesc(group["lr"], b1, b2, group["eps"], group["weight_decay"],
+                                 self.seed, self.state_bits)
+            with _on(dev):
+                check(lib.race_adamw(desc, table, len(params), _raw_stream(dev.index)))
+            for st in live:
+                st["step"] += 1
+        return loss
