@@ -14,7 +14,24 @@
 // k_mm_split: one 128 x NT tile per cluster of C CTAs which split the contraction;
 // the weight (b) takes the M side of the instruction, so that few tokens waste
 // little of it, and the C partial tiles are joined over distributed shared
-// memory in the order of the ranks.  Few launches' worth of tiles, or few rows, go here.
+// memory in the order of the ranks.  Products with few rows or few tiles go here.
+//
+// k_mm_pair: persistent pairs of CTAs, 256 x 256 tiles (tcgen05.mma.cta_group::2: each CTA
+// brings 128 rows of both operands, so a block costs 32 KB of loads where a
+// lone CTA's 128 x 256 tile costs 48).  Warp 0 loads, warp 1 of the first CTA issues the
+// instructions, eight warps promote: a thread sums half a row of the tile, 128
+// columns, in registers.  A block takes the tensor core 450 cycles (four
+// instructions of 112) and the promotion 420, most of it loads from tensor memory;
+// tensor memory holds two accumulators, so one block is promoted while the
+// next is multiplied.  What bounds it is the way round: a block's completion takes
+// about 300 cycles to be seen by the promoting warps of both CTAs, the second
+// CTA's arrival as long to come back, so a block takes 950.  Waits are four
+// instructions long because each stands in that way.  Measured, 16384 x 8192 x 4096:
+// 501 us from a cold start (2193 TFLOP/s, 1965 MHz), 580 us kept up (1897,
+// 1485 MHz under the 1000 W cap); k_mm_split takes 1551 there.  Sixteen promoting
+// warps took 637 (they share the schedulers with the issuing warp), halves of 128
+// columns with four accumulators 869 (twice the waits).  Results leave through
+// shared memory by TMA, 128 bytes of a row at a time.
 #include <atomic>
 
 #include "race_api.h"
@@ -64,6 +81,43 @@ __device__ __forceinline__ void tma2(uint32_t dst, const CUtensorMap* map, int c
       "{%2, %3}], [%4];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
       : "memory");
+}
+
+// One lane of a converged warp.  The code behind it keeps its descriptors and
+// addresses in uniform registers, which the tensor core's and the copy engine's
+// instructions take: behind `lane == 0` each instruction costs 70 cycles of
+// moves instead.
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
+// Up to 64 polls in a loop of four instructions: the warps share their
+// scheduler with promoting ones, each instruction of a wait costs them a turn.
+__device__ __forceinline__ bool spin(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 64;\n"
+      "AGAIN:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra THROUGH;\n\t"
+      "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra AGAIN;\n"
+      "THROUGH:\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait; gives up early once another thread has (see bar_wait).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, int polls) {
+  if (polls >= 64) {
+    if (spin(bar, parity)) return true;
+    for (int i = 64; i < polls && *abort == 0; i += 64)
+      if (spin(bar, parity)) return true;
+    *abort = 1;
+    return false;
+  }
+  return bar_wait(reinterpret_cast<uint64_t*>(__cvta_shared_to_generic(bar)), parity, abort, polls);
 }
 
 __device__ __forceinline__ void bar_arrive(uint64_t* bar) {
@@ -173,9 +227,13 @@ __global__ void __launch_bounds__(kSplitThreads)
         tma2(dst, &mapw, (k0 + i) * 128, (int)n0, saddr(full + s));
         tma2(dst + L::A, &mapx, (k0 + i) * 128, (int)m0, saddr(full + s));
       }
-      if (i < blocks)                                              // gave up: copies in flight land first
+      if (i < blocks) {                                            // gave up: copies in flight land first
         for (int j = i > L::S ? i - L::S : 0; j < i; ++j)
           if (!bar_wait(full + j % L::S, (j / L::S) & 1)) report(a.status, t5::kErrStuck);
+      } else {                                                     // the last commits have arrived
+        for (int j = i > L::S ? i - L::S : 0; j < i; ++j)
+          if (!bar_wait(empty + j % L::S, (j / L::S) & 1, abort, a.polls)) break;
+      }
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -320,6 +378,449 @@ int launch_split(const Args& a, const CUtensorMap& mw, const CUtensorMap& mx, bo
   return e == cudaSuccess ? RACE_OK : api_cuda_fail(e);
 }
 
+// ------------------------------------------------------------------ pairs of CTAs
+
+struct PairArgs {
+  Args a;
+  int tiles_m, tiles_n;    // 256 x 256 tiles
+  int splits;              // of the contraction
+  float* part;             // splits > 1: [split][m][n] partial results
+  int store;               // 1: results leave by TMA (map y), 0: element by element
+};
+
+constexpr int kPairThreads = 384;                                  // a warpgroup that loads and issues, two that promote
+constexpr int kGroup = 8;                                          // row tiles walked together
+
+template <bool SQ>
+struct Pair {
+  static constexpr int A = 128 * 128, STAGE = 2 * A;               // this CTA's rows of a and of b
+  static constexpr int S = SQ ? 5 : 4;
+  static constexpr int OUT = S * STAGE;                            // [8 warps][2] boxes of 32 x 128 bytes
+  static constexpr int SCALES = OUT + 16 * 4096;                   // [2][256] floats (rows of b)
+  static constexpr int BARS = SCALES + (SQ ? 0 : 2048);            // full, empty [S]; tfull, tempty [2]; drain
+  static constexpr int MISC = BARS + (2 * S + 5) * 8;              // tmem base, abort word, loads issued
+  static constexpr int BYTES = MISC + 16 + 1024;
+  static_assert(BYTES <= 232448, "227 KB of shared memory");
+};
+
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t p;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
+  return p;
+}
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+// into this CTA's shared memory, counted by a barrier of either CTA of the pair
+__device__ __forceinline__ void tma2_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma2_store(const CUtensorMap* map, int c0, int c1, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(src)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc));
+}
+// one arrival at the same barrier of both CTAs once the instructions so far are done
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          saddr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+struct Item {
+  int m, n, k0, k1, split;
+};
+__device__ __forceinline__ Item item_of(const PairArgs& p, int i) {
+  const int tiles = p.tiles_m * p.tiles_n;
+  Item t;
+  t.split = i / tiles;
+  const int r = i - t.split * tiles;
+  const int g = r / (kGroup * p.tiles_n), first = g * kGroup;
+  const int rows = min(kGroup, p.tiles_m - first), l = r - first * p.tiles_n;
+  t.m = first + l % rows;
+  t.n = l / rows;
+  t.k0 = (int)((int64_t)p.a.kb * t.split / p.splits);
+  t.k1 = (int)((int64_t)p.a.kb * (t.split + 1) / p.splits);
+  return t;
+}
+
+template <bool SQ>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    k_mm_pair(const __grid_constant__ CUtensorMap mapa, const __grid_constant__ CUtensorMap mapb,
+              const __grid_constant__ CUtensorMap mapy, const PairArgs p) {
+  using L = Pair<SQ>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = raw + ((1024 - (saddr(raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::BARS);
+  uint64_t* empty = full + L::S;
+  uint64_t* tfull = empty + L::S;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::MISC);
+  volatile uint32_t* abort = misc + 1;
+  const Args& a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  const int items = p.tiles_m * p.tiles_n * p.splits;
+
+  if (tid == 0) {
+    for (int i = 0; i < L::S; ++i) {
+      bar_init_n(full + i, 1);
+      bar_init_n(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init_n(tfull + i, 1);
+      bar_init_n(tempty + i, 16);                                  // eight warps of both CTAs
+    }
+    bar_init(drain);
+    misc[1] = 0;
+    misc[2] = 0;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(misc)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  cluster_sync();
+  fence_after();
+  const uint32_t tm = misc[0];
+
+  // 384 x 168 registers at launch = 128 x 40 + 256 x 232
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    const uint32_t full0 = saddr(full), empty0 = saddr(empty);
+    int s = 0;                                                     // stage, and its barriers' phase
+    uint32_t ph = 0;
+    bool ok = true;
+    if (warp == 0) {
+      const uint32_t dst = saddr(sm), bar0 = map_rank(full0, 0);
+      int it = 0;
+      for (int i = cluster; ok && i < items; i += clusters) {
+        const Item t = item_of(p, i);
+        const int ra = t.m * 256 + (int)rank * 128, rb = t.n * 256 + (int)rank * 128;
+        for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
+          if (it >= L::S) ok = wait(empty0 + 8 * s, ph ^ 1, abort, a.polls);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          if (elect()) {
+            if (rank == 0) bar_expect_tx(full + s, 2 * L::STAGE);
+            tma2_pair(dst + s * L::STAGE, &mapa, kb * 128, ra, bar0 + 8 * s);
+            tma2_pair(dst + s * L::STAGE + L::A, &mapb, kb * 128, rb, bar0 + 8 * s);
+          }
+          __syncwarp();
+          if (++s == L::S) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      if (lane == 0) misc[2] = it;
+      // the last commits reach this CTA's barriers before it leaves
+      for (int j = it > L::S ? it - L::S : 0; ok && j < it; ++j)
+        ok = wait(empty0 + 8 * (j % L::S), (j / L::S) & 1, abort, a.polls);
+    } else if (warp == 1 && rank == 0) {
+      const uint64_t da = t5::desc_sw128(sm, 0), db = t5::desc_sw128(sm + L::A, 0);
+      const uint32_t tempty0 = saddr(tempty);
+      int it = 0;
+      for (int i = cluster; ok && i < items; i += clusters) {
+        const Item t = item_of(p, i);
+        for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
+          const int b = it & 1;
+          ok = wait(full0 + 8 * s, ph, abort, a.polls) &&
+               (it < 2 || wait(tempty0 + 8 * b, ((it >> 1) - 1) & 1, abort, a.polls));
+          if (!__all_sync(0xffffffffu, ok)) break;
+          fence_after();
+          if (elect()) {
+            // a stage is 16-byte units further on, a K = 32 step 32 bytes inside the swizzle atom
+            const uint64_t at = (uint64_t)(s * (L::STAGE >> 4));
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              mma8_pair(tm + b * 256, da + at + 2 * ks, db + at + 2 * ks, idesc8<256, 256>(), ks > 0);
+            commit_pair(tfull + b);
+            commit_pair(empty + s);
+          }
+          __syncwarp();
+          if (++s == L::S) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      if (!ok) {
+        if (elect()) commit_pair(drain);
+        __syncwarp();
+        if (!bar_wait(drain, 0) && lane == 0) report(a.status, t5::kErrStuck);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int quarter = warp & 3, part = (warp - 4) >> 2, row = 32 * quarter + lane;
+    const uint32_t lanes = tm + ((uint32_t)(32 * quarter) << 16) + 128 * part;
+    const uint32_t te = map_rank(saddr(tempty), 0), tf = saddr(tfull);
+    uint8_t* box = sm + L::OUT + (warp - 4) * 8192;
+    float* sbs = reinterpret_cast<float*>(sm + L::SCALES) + 128 * part;
+    int it = 0;
+    for (int i = cluster; i < items; i += clusters) {
+      const Item t = item_of(p, i);
+      const int64_t mr = (int64_t)t.m * 256 + rank * 128 + row;    // this thread's row of the result
+      const int64_t n0 = (int64_t)t.n * 256 + 128 * part;           // its first column
+      const float* sa = a.sa + (mr < a.m ? mr : a.m - 1) * a.sar;
+      // square: one scale for the 128 columns; else thread `row` fetches that of column `row`
+      const int64_t br = SQ ? min(n0, a.n - 1) / 128 : min(n0 + row, a.n - 1);
+      const float* sb = a.sb + br * a.sbr;
+      float acc[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      float na = __ldg(sa + t.k0 * a.sab), nb = __ldg(sb + t.k0 * a.sbb);
+      for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
+        const int b = it & 1;
+        const float ca = na, cb = nb;
+        const float* sbb = sbs + 256 * b;
+        if constexpr (!SQ) {
+          sbs[256 * b + row] = cb;
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");   // the four warps of these columns
+        }
+        if (kb + 1 < t.k1) {
+          na = __ldg(sa + (kb + 1) * a.sab);
+          nb = __ldg(sb + (kb + 1) * a.sbb);
+        }
+        // a wait that ran out leaves garbage here, which is not stored
+        wait(tf + 8 * b, (it >> 1) & 1, abort, a.polls);
+        __syncwarp();
+        fence_after();
+        const float sc = ca * cb;
+        // the next 16 columns are on their way while these are added
+        float v[2][16];
+        t5::tld16(lanes + b * 256, v[0]);
+#pragma unroll
+        for (int c = 0; c < 128; c += 16) {
+          const int cur = (c >> 4) & 1;
+          t5::tld_wait();
+          if (c < 112) {
+            t5::tld16(lanes + b * 256 + c + 16, v[cur ^ 1]);
+          } else {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_at(te + 8 * b);
+          }
+#pragma unroll
+          for (int q = 0; q < 16; q += 2) {
+            float2 s2 = make_float2(sc, sc);
+            if constexpr (!SQ) {
+              const float2 w = *reinterpret_cast<const float2*>(sbb + c + q);
+              s2 = __fmul2_rn(make_float2(ca, ca), w);
+            }
+            const float2 r = __ffma2_rn(s2, make_float2(v[cur][q], v[cur][q + 1]),
+                                        make_float2(acc[c + q], acc[c + q + 1]));
+            acc[c + q] = r.x;
+            acc[c + q + 1] = r.y;
+          }
+        }
+      }
+      if (*abort != 0) continue;
+      if (p.splits > 1) {
+        // partial results are read once, by the join
+        float* o = p.part + ((int64_t)t.split * a.m + mr) * a.n + n0;
+        if (mr < a.m) {
+          if (n0 + 128 <= a.n && a.n % 4 == 0) {
+#pragma unroll
+            for (int j = 0; j < 128; j += 4)
+              *reinterpret_cast<float4*>(o + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+              if (n0 + j < a.n) o[j] = acc[j];
+          }
+        }
+      } else if (p.store) {
+        // 128 bytes of 32 rows at a time, 16-byte chunk c of row r at c ^ (r % 8)
+        const int es = a.ybf16 ? 2 : 4;
+        const int r0 = (int)(mr - lane);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (a.ybf16 && g >= 2) break;
+          uint8_t* o = box + 4096 * (g & 1);
+          if (lane == 0) store_wait_read<1>();                     // the box's last store has read it
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint4 u;
+            if (a.ybf16) {
+              uint32_t w[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int j = (g & 1) * 64 + 8 * c + 2 * q;
+                const __nv_bfloat162 h = __floats2bfloat162_rn(acc[j], acc[j + 1]);
+                w[q] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+              u = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+              const int j = g * 32 + 4 * c;
+              u = make_uint4(__float_as_uint(acc[j]), __float_as_uint(acc[j + 1]),
+                             __float_as_uint(acc[j + 2]), __float_as_uint(acc[j + 3]));
+            }
+            *reinterpret_cast<uint4*>(o + lane * 128 + ((c ^ (lane & 7)) << 4)) = u;
+          }
+          t5::fence_async_smem();
+          __syncwarp();
+          const int64_t col = n0 + g * (128 / es);
+          if (lane == 0) {
+            if (col < a.n && r0 < a.m) tma2_store(&mapy, (int)(col * es), r0, saddr(o));
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // one group a box, stored or not
+          }
+        }
+      } else if (mr < a.m) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+          if (n0 + j < a.n) put(a, mr, n0 + j, acc[j]);
+      }
+    }
+    if (lane == 0) store_wait_read<0>();
+  }
+  __syncthreads();
+  cluster_sync();
+  const bool mine = *abort != 0;
+  if (mine && tid == 0) report(a.status, t5::kErrTimeout);
+  // Copies in flight land before either CTA leaves: the first CTA's barriers
+  // count both CTAs' bytes, so it settles what only one of them issued.
+  const uint32_t other = ld_cluster_u32(map_rank(saddr(misc + 1), rank ^ 1));
+  if (rank == 0 && tid == 0 && (mine || other != 0)) {
+    const int i0 = (int)misc[2], i1 = (int)ld_cluster_u32(map_rank(saddr(misc + 2), 1));
+    const int lo = min(i0, i1), hi = max(i0, i1);
+    for (int j = lo; j < hi; ++j) {
+      uint64_t* f = full + j % L::S;
+      if (j < i0)
+        asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(saddr(f)),
+                     "r"(L::STAGE)
+                     : "memory");
+      else
+        bar_expect_tx(f, L::STAGE);
+    }
+    for (int j = hi > L::S ? hi - L::S : 0; j < hi; ++j)
+      if (!bar_wait(full + j % L::S, (j / L::S) & 1)) report(a.status, t5::kErrStuck);
+  }
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tm));
+}
+
+// result = sum over the splits of their partial results, in their order
+__global__ void __launch_bounds__(256) k_mm_join(const float* __restrict__ part, int splits, const Args a) {
+  const int64_t total = a.m * a.n;
+  const int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  if (i >= total) return;
+  if (total % 4 == 0) {                      // then every split starts on 16 bytes
+    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < splits; ++s) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(part + s * total + i));
+      t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+    }
+    const float r[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) put(a, (i + j) / a.n, (i + j) % a.n, r[j]);
+  } else {
+    for (int64_t e = i; e < i + 4 && e < total; ++e) {
+      float t = 0.f;
+      for (int s = 0; s < splits; ++s) t += part[s * total + e];
+      put(a, e / a.n, e % a.n, t);
+    }
+  }
+}
+
+template <bool SQ>
+int launch_pair(const PairArgs& p, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& my,
+                cudaStream_t s) {
+  static std::atomic<uint64_t> ready;
+  RACE_CALL(allow_smem(reinterpret_cast<const void*>(&k_mm_pair<SQ>), Pair<SQ>::BYTES, ready));
+  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  const int64_t pairs = api_sm_count() / 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2u * (unsigned)(items < pairs ? items : pairs));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = Pair<SQ>::BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, &k_mm_pair<SQ>, ma, mb, my, p);
+  api_log("mm_pair");
+  if (e == cudaSuccess && p.splits > 1) {
+    const int64_t quads = (p.a.m * p.a.n + 3) / 4;
+    k_mm_join<<<(unsigned)((quads + 255) / 256), 256, 0, s>>>(p.part, p.splits, p.a);
+    api_log("mm_join");
+    e = cudaGetLastError();
+  }
+  return e == cudaSuccess ? RACE_OK : api_cuda_fail(e);
+}
+
+// How a product is cut.  Measured on 148 SMs, in the time of one block on a
+// pair (512 cycles of its tensor core): see the comment at each figure.
+struct Plan {
+  bool pair;
+  int nt, c;               // k_mm_split: token columns of a tile, CTAs of a cluster
+  int tiles_m, tiles_n, splits;
+};
+
+Plan plan_of(int64_t m, int64_t n, int64_t k) {
+  Plan p{};
+  const int64_t kb = (k + 127) / 128, sms = api_sm_count();
+  p.nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+  p.c = 1;
+  const int64_t tiles = ((n + 127) / 128) * ((m + p.nt - 1) / p.nt);
+  while (p.c < 8 && tiles * p.c * 2 <= 2 * sms && p.c * 2 <= kb) p.c *= 2;
+  p.tiles_m = (int)((m + 255) / 256);
+  p.tiles_n = (int)((n + 255) / 256);
+  p.splits = 1;
+  const int64_t big = (int64_t)p.tiles_m * p.tiles_n, pairs = sms / 2;
+  // a whole round of pairs, or a contraction long enough to be cut into one
+  p.pair = m > 128 && n > 128 && (big >= pairs || big * (kb / 16) >= pairs);
+  if (p.pair && big < 4 * pairs) {
+    // rounds of the pairs times blocks of an item, plus the partial results'
+    // way to memory and back
+    double best = 1e30;
+    for (int s = 1; s <= 32 && s <= kb; ++s) {
+      const double rounds = (double)((big * s + pairs - 1) / pairs);
+      const double cost = rounds * ((double)((kb + s - 1) / s) + 3.0) +
+                          (s > 1 ? 8.0 + s * (double)(m * n) * 1.6e-6 * 4 : 0.0);
+      if (cost < best) {
+        best = cost;
+        p.splits = s;
+      }
+    }
+  }
+  return p;
+}
+
 int check(const race_matmul_desc_t* d) {
   if (d == nullptr || d->m < 0 || d->n < 0 || d->k < 0 || d->wait_polls < 0) return RACE_ERR_INVALID;
   if (d->out_dtype != RACE_F32 && d->out_dtype != RACE_BF16) return RACE_ERR_INVALID;
@@ -343,14 +844,14 @@ int check_operand(race_blocks_t b, int64_t rows, int64_t k) {
 using namespace race;
 
 extern "C" size_t race_scaled_matmul_workspace(const race_matmul_desc_t* desc) {
-  return mm::check(desc) == RACE_OK ? 0 : 0;
+  if (mm::check(desc) != RACE_OK || desc->m == 0 || desc->n == 0 || desc->k == 0) return 0;
+  const mm::Plan p = mm::plan_of(desc->m, desc->n, desc->k);
+  return p.pair && p.splits > 1 ? (size_t)p.splits * (size_t)desc->m * (size_t)desc->n * sizeof(float) : 0;
 }
 
 extern "C" int race_scaled_matmul(const race_matmul_desc_t* desc, race_blocks_t a, race_blocks_t b,
                                   race_rows_t result, uint32_t* status, void* workspace,
                                   size_t workspace_bytes, cudaStream_t stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   ApiCall call;
   RACE_CALL(mm::check(desc));
   if (desc->m == 0 || desc->n == 0) return RACE_OK;
@@ -368,23 +869,35 @@ extern "C" int race_scaled_matmul(const race_matmul_desc_t* desc, race_blocks_t 
   mm::Args g{a.scales, a.stride_row, a.stride_block, b.scales, b.stride_row, b.stride_block,
              result.data, result.ld, desc->out_dtype == RACE_BF16, desc->m, desc->n,
              (int)((desc->k + 127) / 128), desc->wait_polls > 0 ? desc->wait_polls : mm::kPolls, status};
-  const int nt = desc->m <= 16 ? 16 : desc->m <= 32 ? 32 : desc->m <= 64 ? 64 : 128;
-  CUtensorMap mw, mx;
-  if (!api_encode_bytes(&mw, b.codes, desc->n, desc->k, b.ld, 128) ||
-      !api_encode_bytes(&mx, a.codes, desc->m, desc->k, a.ld, nt))
-    return RACE_ERR_UNSUPPORTED;
-  // split the contraction while the tiles leave SMs idle
-  const int64_t tiles = ((desc->n + 127) / 128) * ((desc->m + nt - 1) / nt);
-  int c = 1;
-  while (c < 8 && tiles * c * 2 <= 2 * (int64_t)api_sm_count() && c * 2 <= g.kb) c *= 2;
-  if ((desc->m + nt - 1) / nt > 65535 || (desc->n + 127) / 128 > 65535) {
+  const mm::Plan plan = mm::plan_of(desc->m, desc->n, desc->k);
+  const bool square = desc->b_square != 0;
+  CUtensorMap ma, mb;
+  if (plan.pair) {
+    const size_t need = plan.splits > 1 ? (size_t)plan.splits * desc->m * desc->n * sizeof(float) : 0;
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return RACE_ERR_WORKSPACE;
+    CUtensorMap my;
+    const bool store = reinterpret_cast<uintptr_t>(result.data) % 16 == 0 && result.ld * es % 16 == 0;
+    if (!api_encode_bytes(&ma, a.codes, desc->m, desc->k, a.ld, 128) ||
+        !api_encode_bytes(&mb, b.codes, desc->n, desc->k, b.ld, 128) ||
+        !(store ? api_encode_bytes(&my, result.data, desc->m, desc->n * es, result.ld * es, 32)
+                : api_encode_bytes(&my, a.codes, desc->m, desc->k, a.ld, 32)))
+      return RACE_ERR_UNSUPPORTED;
+    const mm::PairArgs p{g, plan.tiles_m, plan.tiles_n, plan.splits, static_cast<float*>(workspace), store};
+    return square ? mm::launch_pair<true>(p, ma, mb, my, stream)
+                  : mm::launch_pair<false>(p, ma, mb, my, stream);
+  }
+  const int64_t tm = (desc->m + plan.nt - 1) / plan.nt, tn = (desc->n + 127) / 128;
+  if (tm > 65535 || tn > 65535) {
     api_note("matmul: more than 65535 tiles along one side");
     return RACE_ERR_UNSUPPORTED;
   }
-  switch (nt) {
-    case 16: return mm::launch_split<16>(g, mw, mx, desc->b_square != 0, c, stream);
-    case 32: return mm::launch_split<32>(g, mw, mx, desc->b_square != 0, c, stream);
-    case 64: return mm::launch_split<64>(g, mw, mx, desc->b_square != 0, c, stream);
-    default: return mm::launch_split<128>(g, mw, mx, desc->b_square != 0, c, stream);
+  if (!api_encode_bytes(&mb, b.codes, desc->n, desc->k, b.ld, 128) ||
+      !api_encode_bytes(&ma, a.codes, desc->m, desc->k, a.ld, plan.nt))
+    return RACE_ERR_UNSUPPORTED;
+  switch (plan.nt) {
+    case 16: return mm::launch_split<16>(g, mb, ma, square, plan.c, stream);
+    case 32: return mm::launch_split<32>(g, mb, ma, square, plan.c, stream);
+    case 64: return mm::launch_split<64>(g, mb, ma, square, plan.c, stream);
+    default: return mm::launch_split<128>(g, mb, ma, square, plan.c, stream);
   }
 }
