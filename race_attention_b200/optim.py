@@ -10,9 +10,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib
-from ._lib import RaceAdamwDesc, RaceAdamwTensor, check
-from .fp8 import BLOCK, F8, _on, _raw_stream
+from .fp8 import BLOCK, F8, _ops
 from .functional import _SUPPORTED
 
 
@@ -41,9 +39,9 @@ class AdamW(torch.optim.Optimizer):
         self._check_group({"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay})
         self.state_bits = state_bits
         self.seed = int(seed) & 0xFFFFFFFF
-        self.offsets, self._sizes = {}, {}
+        self.offsets = {}
         self._total = 0
-        self._tables = {}
+        self._plans = []          # of each group: where its states begin, sizes, steps taken
         self.exp_avg = self.exp_avg_sq = None
         self.exp_avg_scale = self.exp_avg_sq_scale = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
@@ -75,11 +73,13 @@ class AdamW(torch.optim.Optimizer):
         before = self._total
         for p in group["params"]:
             self.offsets[p] = self._total
-            self._sizes[p] = p.numel()
             self._total += -(-p.numel() // BLOCK) * BLOCK
-            self.state[p]["step"] = 0
+        params = group["params"]
+        steps = torch.zeros(len(params), dtype=torch.int32)
+        self._plans.append(([self.offsets[p] for p in params], [p.numel() for p in params], steps))
+        for p, s in zip(params, steps):
+            self.state[p]["step"] = s      # a view: the step counts it up
         self._grow(self._total - before)
-        self._tables.clear()
 
     def _device(self, group) -> torch.device:
         for g in self.param_groups:
@@ -118,9 +118,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"{name} must be a contiguous tensor like this optimizer's own")
         self.exp_avg, self.exp_avg_sq = exp_avg, exp_avg_sq
         self.exp_avg_scale, self.exp_avg_sq_scale = exp_avg_scale, exp_avg_sq_scale
-        for s in self.state.values():
-            s["step"] = int(step)
-        self._tables.clear()
+        for _, _, steps in self._plans:
+            steps.fill_(int(step))
 
     def state_dict(self):
         groups, index = [], {}
@@ -129,7 +128,7 @@ class AdamW(torch.optim.Optimizer):
                 index[p] = len(index)
             groups.append({**{k: v for k, v in g.items() if k != "params"},
                            "params": [index[p] for p in g["params"]]})
-        return {"state": {index[p]: {"step": self.state[p]["step"], "first": self.offsets[p]} for p in index},
+        return {"state": {index[p]: {"step": int(self.state[p]["step"]), "first": self.offsets[p]} for p in index},
                 "param_groups": groups, "state_bits": self.state_bits, "seed": self.seed,
                 "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq,
                 "exp_avg_scale": self.exp_avg_scale, "exp_avg_sq_scale": self.exp_avg_sq_scale}
@@ -150,27 +149,10 @@ class AdamW(torch.optim.Optimizer):
         self.set_state(0, *(None if state_dict[n] is None else state_dict[n].to(dev, copy=True)
                             for n in names))
         for i, p in zip(order, params):
-            self.state[p]["step"] = int(state_dict["state"][i]["step"])
+            self.state[p]["step"].fill_(int(state_dict["state"][i]["step"]))
         for g, s in zip(self.param_groups, groups):
             g.update({k: v for k, v in s.items() if k != "params"})
         self.seed = int(state_dict["seed"]) & 0xFFFFFFFF
-
-    def _table(self, gi: int, params):
-        """The C array of a group's tensors, its constant fields filled in."""
-        t = self._tables.get(gi)
-        if t is None:
-            t = (RaceAdamwTensor * len(params))()
-            m, v = self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr()
-            size = self.exp_avg.element_size()
-            for e, p in zip(t, params):
-                at = self.offsets[p]
-                e.exp_avg, e.exp_avg_sq = m + at * size, v + at * size
-                if self.state_bits == 8:
-                    e.exp_avg_scale = self.exp_avg_scale.data_ptr() + at // BLOCK * 4
-                    e.exp_avg_sq_scale = self.exp_avg_sq_scale.data_ptr() + at // BLOCK * 4
-                e.first = at
-            self._tables[gi] = t
-        return t
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -178,39 +160,9 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        lib = _lib.load()
-        dev = self.exp_avg.device
-        for gi, group in enumerate(self.param_groups):
-            params = group["params"]
-            table = self._table(gi, params)
-            kept, live = [], []       # gradients copied for this step, tensors that move
-            for e, p in zip(table, params):
-                g = p.grad
-                if g is None:
-                    e.numel = 0
-                    continue
-                if g.dtype != p.dtype or g.is_sparse or g.device != p.device:
-                    raise ValueError("gradients must be dense, on their parameter's device and of its type")
-                n = p.numel()
-                if not p.is_contiguous() or n != self._sizes[p] or p.device != dev \
-                        or p.dtype not in _SUPPORTED:
-                    raise ValueError("a parameter changed its size, layout, type or device since "
-                                     "the optimizer was built")
-                if not g.is_contiguous():
-                    g = g.contiguous()
-                    kept.append(g)
-                st = self.state[p]
-                e.param, e.grad, e.numel = p.data_ptr(), g.data_ptr(), n
-                e.dtype = _lib.RACE_F32 if p.dtype == torch.float32 else _lib.RACE_BF16
-                e.step = st["step"]
-                live.append(st)
-            if not live:
-                continue
+        for group, (first, sizes, steps) in zip(self.param_groups, self._plans):
             b1, b2 = group["betas"]
-            desc = RaceAdamwDesc(group["lr"], b1, b2, group["eps"], group["weight_decay"],
-                                 self.seed, self.state_bits)
-            with _on(dev):
-                check(lib.race_adamw(desc, table, len(params), _raw_stream(dev.index)))
-            for st in live:
-                st["step"] += 1
+            _ops.adamw(group["params"], first, sizes, steps, self.exp_avg, self.exp_avg_sq,
+                       self.exp_avg_scale, self.exp_avg_sq_scale, group["lr"], b1, b2, group["eps"],
+                       group["weight_decay"], self.seed, self.state_bits)
         return loss

@@ -98,7 +98,7 @@ def test_adamw_arguments(lib):
     assert lib.race_adamw(d(), None, 2, None) == INVALID
 
 
-def test_python_refusals_on_the_host():
+def test_python_refusals_on_the_host(lib):
     from race_attention_b200.fp8 import BlockFp8, fp8_matmul, quantize_fp8, rms_norm
     x = torch.ones(3, 200)
     for f in (lambda: quantize_fp8(x), lambda: rms_norm(x, torch.ones(200))):

@@ -237,7 +237,7 @@ def test_product_on_another_stream_and_in_a_graph():
 def test_product_wait_limit(m):
     """A wait that runs out is reported, and the next call is whole again."""
     from race_attention_b200 import _lib
-    from race_attention_b200.fp8 import _rb, _rr, fp8_matmul
+    from race_attention_b200.fp8 import fp8_matmul
     a, b = operands(m, 640, 1280, True, seed=6)
     A, B = held(*a), held(*b)
     ref = fp8_matmul(A, B)
@@ -247,8 +247,11 @@ def test_product_wait_limit(m):
     desc = _lib.RaceMatmulDesc(_lib.RACE_BF16, 1, m, 640, 1280, 1, 0)
     need = lib.race_scaled_matmul_workspace(desc)
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
-    _lib.check(lib.race_scaled_matmul(desc, _rb(A), _rb(B), _rr(out), word.data_ptr(), ws.data_ptr(),
-                                      need, torch.cuda.current_stream().cuda_stream))
+    blocks = lambda b: _lib.RaceBlocks(b.codes.data_ptr(), b.codes.stride(0), b.scales.data_ptr(),  # noqa: E731
+                                       *b.scales.stride())
+    _lib.check(lib.race_scaled_matmul(desc, blocks(A), blocks(B), _lib.RaceRows(out.data_ptr(), 640),
+                                      word.data_ptr(), ws.data_ptr(), need,
+                                      torch.cuda.current_stream().cuda_stream))
     torch.cuda.synchronize()
     assert int(word) & _lib.RACE_DEV_TIMEOUT and not int(word) & _lib.RACE_DEV_STUCK
     assert torch.equal(fp8_matmul(A, B), ref)
