@@ -60,11 +60,12 @@ struct Args {
   Item item[N];
 };
 
+// h of the noise h ^ (h >> 16): its upper half is h's own
 __device__ __forceinline__ uint32_t noise(uint32_t i, uint32_t key) {
-  uint32_t h = (i ^ key) * kGolden;
-  h = (h ^ (h >> 15)) * kRootTwo;
-  return h ^ (h >> 16);
+  const uint32_t h = (i ^ key) * kGolden;
+  return (h ^ (h >> 15)) * kRootTwo;
 }
+__device__ __forceinline__ uint32_t lower(uint32_t h) { return (h ^ (h >> 16)) & 0xffffu; }
 
 // y in [0, 448] up or down to the 8-bit format, r16 of 65536ths deciding: below
 // 2^-6 the format's steps are even, as they are for every number of the binade
@@ -122,7 +123,7 @@ __device__ __forceinline__ void hold(void* p, float* scales, int64_t at, bool li
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float y = fminf(fabsf(x[i]) * inv, kTop);
-    float d = dither(y, ROOT ? r[i] >> 16 : r[i] & 0xffffu);
+    float d = dither(y, ROOT ? r[i] >> 16 : lower(r[i]));
     if (ROOT && d == 0.f && y > 0.f) d = 0.001953125f;
     c[i] = ROOT ? d : copysignf(d, x[i]);
   }
@@ -177,7 +178,11 @@ __global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a)
     m[i] = __fadd_rn(__fmul_rn(a.b1, m[i]), __fmul_rn(a.c1, g[i]));
     v[i] = __fadd_rn(__fmul_rn(a.b2, v[i]), __fmul_rn(__fmul_rn(a.c2, g[i]), g[i]));
     root[i] = sqrtf(v[i]);
-    p[i] = fmaf(-it.step_size, m[i] / fmaf(root[i], it.root_scale, a.eps), p[i] * a.keep);
+    const float den = fmaf(root[i], it.root_scale, a.eps);
+    // with 8-bit states arithmetic is the bound: the quotient may be two units of
+    // its last place off, far inside a step of either format
+    const float q = EIGHT ? __fdividef(m[i], den) : m[i] / den;
+    p[i] = fmaf(-it.step_size, q, p[i] * a.keep);
   }
   if (half) {
 #pragma unroll
@@ -185,7 +190,7 @@ __global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a)
       const uint32_t b = __float_as_uint(p[i]);
       // infinities and NaN keep their bits
       if ((b & 0x7f800000u) != 0x7f800000u)
-        p[i] = __uint_as_float((b + (noise(i0 + i, it.key + 1) & 0xffffu)) & ~0xffffu);
+        p[i] = __uint_as_float((b + lower(noise(i0 + i, it.key + 1))) & ~0xffffu);
     }
     store_some(static_cast<bf16*>(it.p) + at, vec, n, p);
   } else {

@@ -28,8 +28,79 @@ struct Args {
 
 constexpr int NT = 256;
 
+// The thread's 8 x 8 values.  bfloat16 stays packed (32 registers in place of
+// 64, which lets three CTAs share an SM) and its maxima are taken two at a time.
+template <typename T>
+struct Tile;
+
+template <>
+struct Tile<float> {
+  float v[8][8];
+  __device__ __forceinline__ void load(int i, const float* p) { load8(p, v[i]); }
+  __device__ __forceinline__ void set(int i, int j, float x) { v[i][j] = x; }
+  __device__ __forceinline__ float get(int i, int j) const { return v[i][j]; }
+  __device__ __forceinline__ uint32_t row_max(int i) const {
+    uint32_t m = mag(v[i][0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = max(m, mag(v[i][j]));
+    return m;
+  }
+  __device__ __forceinline__ void col_max(uint32_t (&m)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m[j] = mag(v[0][j]);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) m[j] = max(m[j], mag(v[i][j]));
+    }
+  }
+};
+
+template <>
+struct Tile<bf16> {
+  uint32_t w[8][4];
+  __device__ __forceinline__ void load(int i, const bf16* p) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
+  }
+  __device__ __forceinline__ void set(int i, int j, float x) {
+    const uint32_t b = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(x));
+    w[i][j >> 1] = (j & 1) ? (w[i][j >> 1] & 0xffffu) | b << 16 : b;   // even columns are set first
+  }
+  __device__ __forceinline__ float get(int i, int j) const {
+    return __uint_as_float((j & 1) ? w[i][j >> 1] & 0xffff0000u : w[i][j >> 1] << 16);
+  }
+  // the larger magnitudes of two pairs, NaN if there is one
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmax2_nan(__habs2(reinterpret_cast<const __nv_bfloat162&>(a)),
+                                         __habs2(reinterpret_cast<const __nv_bfloat162&>(b)));
+    return reinterpret_cast<const uint32_t&>(r);
+  }
+  __device__ __forceinline__ uint32_t row_max(int i) const {
+    const uint32_t m = max2(max2(w[i][0], w[i][1]), max2(w[i][2], w[i][3]));
+    return max(m & 0x7fff0000u, m << 16 & 0x7fff0000u);
+  }
+  __device__ __forceinline__ void col_max(uint32_t (&m)[8]) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t t = w[0][q];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) t = max2(t, w[i][q]);
+      m[2 * q] = t << 16 & 0x7fff0000u;
+      m[2 * q + 1] = t & 0x7fff0000u;
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ uint2 code_row(const Tile<T>& t, int i, float inv) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = t.get(i, j);
+  return code8(v, inv);
+}
+
 template <typename T, bool VEC, bool SQUARE, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(NT) k_quantize(const Args a) {
+__global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_quantize(const Args a) {
   __shared__ __align__(16) uint2 tile[COLS ? 128 * 16 : 1];   // [column][8-row group], swizzled
   __shared__ uint32_t wmax[8][COLS && !SQUARE ? 128 : 1];
   __shared__ float cinv[COLS && !SQUARE ? 128 : 1];
@@ -39,24 +110,45 @@ __global__ void __launch_bounds__(NT) k_quantize(const Args a) {
   const int64_t r0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 128;
   const int64_t r = r0 + 8 * ty, c = c0 + 8 * tx;
   const T* x = static_cast<const T*>(a.x) + r * a.ld + c;
-  float v[8][8];
+  Tile<T> v;
+  if (VEC && r0 + 128 <= a.rows && c0 + 128 <= a.cols) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (VEC && r + i < a.rows && c + 8 <= a.cols) {
-      load8(x + i * a.ld, v[i]);
-    } else {
+    for (int i = 0; i < 8; ++i) v.load(i, x + i * a.ld);
+  } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[i][j] = r + i < a.rows && c + j < a.cols ? to_f32(x[i * a.ld + j]) : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      if (VEC && r + i < a.rows && c + 8 <= a.cols) {
+        v.load(i, x + i * a.ld);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          v.set(i, j, r + i < a.rows && c + j < a.cols ? to_f32(x[i * a.ld + j]) : 0.f);
+      }
     }
   }
-  uint2 code[8];
+  if constexpr (COLS && !SQUARE) {
+    uint32_t m[8];
+    v.col_max(m);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+    if (lane < 16)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) wmax[warp][8 * tx + j] = m[j];
+    __syncthreads();
+    if (tid < 128) {
+      uint32_t t = wmax[0][tid];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) t = max(t, wmax[w][tid]);
+      const float s = scale_of(t);
+      cinv[tid] = 1.f / s;
+      if (c0 + tid < a.cols) a.cs[(c0 + tid) * a.csr + blockIdx.y * a.csb] = s;
+    }
+  }
+  uint2 code[SQUARE ? 8 : 1];
   if constexpr (SQUARE) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, mag(v[i][j]));
+    for (int i = 0; i < 8; ++i) m = max(m, v.row_max(i));
     m = max_over(m, 32);
     if (lane == 0) wmax[warp][0] = m;
     __syncthreads();
@@ -68,48 +160,26 @@ __global__ void __launch_bounds__(NT) k_quantize(const Args a) {
       if (COLS && a.cs != nullptr) a.cs[blockIdx.x * a.csr + blockIdx.y * a.csb] = s;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) code[i] = code8(v[i], inv);
-  } else if constexpr (ROWS) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, mag(v[i][j]));
-      const float s = scale_of(max_over(m, 16));
-      if (tx == 0 && r + i < a.rows) a.rs[(r + i) * a.rsr + blockIdx.x * a.rsb] = s;
-      code[i] = code8(v[i], 1.f / s);
-    }
+    for (int i = 0; i < 8; ++i) code[i] = code_row(v, i, inv);
   }
   if constexpr (ROWS) {
+    // the pitch is a multiple of 16: whole 8-byte groups fit
+    const bool in = c < ((a.cols + 15) & ~int64_t(15));
 #pragma unroll
-    for (int i = 0; i < 8; ++i)   // the pitch is a multiple of 16: whole 8-byte groups fit
-      if (r + i < a.rows && c < ((a.cols + 15) & ~int64_t(15)))
-        *reinterpret_cast<uint2*>(a.rc + (r + i) * a.ldr + c) = code[i];
+    for (int i = 0; i < 8; ++i) {
+      uint2 q;
+      if constexpr (SQUARE) {
+        q = code[i];
+      } else {
+        const float s = scale_of(max_over(v.row_max(i), 16));
+        if (tx == 0 && r + i < a.rows) a.rs[(r + i) * a.rsr + blockIdx.x * a.rsb] = s;
+        q = code_row(v, i, 1.f / s);
+      }
+      if (r + i < a.rows && in) *reinterpret_cast<uint2*>(a.rc + (r + i) * a.ldr + c) = q;
+    }
   }
   if constexpr (COLS) {
-    if constexpr (!SQUARE) {
-      uint32_t m[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        m[j] = mag(v[0][j]);
-#pragma unroll
-        for (int i = 1; i < 8; ++i) m[j] = max(m[j], mag(v[i][j]));
-        m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
-      }
-      if (lane < 16)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) wmax[warp][8 * tx + j] = m[j];
-      __syncthreads();
-      if (tid < 128) {
-        uint32_t t = wmax[0][tid];
-#pragma unroll
-        for (int w = 1; w < 8; ++w) t = max(t, wmax[w][tid]);
-        const float s = scale_of(t);
-        cinv[tid] = 1.f / s;
-        if (c0 + tid < a.cols) a.cs[(c0 + tid) * a.csr + blockIdx.y * a.csb] = s;
-      }
-      __syncthreads();
-    }
+    if constexpr (!SQUARE) __syncthreads();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       uint2 p;
@@ -125,7 +195,7 @@ __global__ void __launch_bounds__(NT) k_quantize(const Args a) {
         const float inv = cinv[8 * tx + j];
         float t[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = v[i][j];
+        for (int i = 0; i < 8; ++i) t[i] = v.get(i, j);
         p = code8(t, inv);
       }
       // lanes of one column group fall on 16 different word pairs
