@@ -418,7 +418,7 @@ typedef struct {
   float* exp_avg_scale;
   float* exp_avg_sq_scale;
   int64_t numel;
-  uint64_t first;         /* index of element 0 in the noise of stochastic rounding */
+  uint64_t first;         /* index of element 0 in the noise of the rounding, a multiple of 8 */
   int32_t dtype;          /* race_dtype_t of param and grad                        */
   int32_t step;           /* steps taken before this one                           */
 } race_adamw_tensor_t;

@@ -61,19 +61,27 @@ struct Args {
 };
 
 // h of the noise h ^ (h >> 16): its upper half is h's own
-__device__ __forceinline__ uint32_t noise(uint32_t i, uint32_t key) {
-  const uint32_t h = (i ^ key) * kGolden;
+__device__ __forceinline__ uint32_t noise(uint32_t i_xor_key) {
+  const uint32_t h = i_xor_key * kGolden;
   return (h ^ (h >> 15)) * kRootTwo;
 }
 __device__ __forceinline__ uint32_t lower(uint32_t h) { return (h ^ (h >> 16)) & 0xffffu; }
 
-// y in [0, 448] up or down to the 8-bit format, r16 of 65536ths deciding: below
-// 2^-6 the format's steps are even, as they are for every number of the binade
-// that adding 2^-6 moves y to.
-__device__ __forceinline__ float dither(float y, uint32_t r16) {
-  const float low = y < 0.015625f ? 0.015625f : 0.f;
-  const uint32_t b = (__float_as_uint(y + low) + (r16 << 4)) & ~0xfffffu;
-  return __uint_as_float(b) - low;
+// y in [0, 448] up or down to the 8-bit format, r of 65536ths deciding (r20 = 16 r):
+// below 2^-6 the format's steps are even, as they are for every number of the
+// binade that adding 2^-6 moves y to.
+__device__ __forceinline__ float dither(float y, uint32_t r20) {
+  const bool low = y < 0.015625f;
+  const float z = low ? y + 0.015625f : y;
+  const float t = __uint_as_float((__float_as_uint(z) + r20) & ~0xfffffu);
+  return low ? t - 0.015625f : t;
+}
+
+// the larger magnitude, NaN if one is
+__device__ __forceinline__ float max_mag(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
 }
 
 template <typename T>
@@ -96,36 +104,57 @@ __device__ __forceinline__ void store_some(T* p, bool vec, int n, const float (&
     if (i < n) p[i] = from_f32<T>(v[i]);
 }
 
+// Pairs of values go through the two-wide multiply and add.
+struct Eight {
+  float2 v[4];
+  __device__ __forceinline__ float get(int i) const { return i & 1 ? v[i >> 1].y : v[i >> 1].x; }
+};
+
+// sums of two products that are rounded first (a two-wide sum would be fused with them)
+__device__ __forceinline__ float2 add_apart(float2 a, float2 b) {
+  return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y));
+}
+
 // eight codes of a state's block (states start on 128-element boundaries, so
 // whole words are always inside them)
-__device__ __forceinline__ void load_codes(const void* p, int64_t at, float s, float (&v)[8]) {
+__device__ __forceinline__ Eight load_codes(const void* p, int64_t at, float s) {
   const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p) + at);
+  Eight e;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t w = i < 2 ? u.x : u.y;
     const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * (i & 1))), __NV_E4M3);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hr));
-    v[2 * i] = f.x * s;
-    v[2 * i + 1] = f.y * s;
+    e.v[i] = __fmul2_rn(__half22float2(*reinterpret_cast<const __half2*>(&hr)), make_float2(s, s));
   }
+  return e;
 }
 
-// Holds a state's eight values of this lane; `upper` picks the half of the noise.
+// Holds a state's eight values of this lane.  ROOT: they are roots, at least
+// zero, and take the upper half of the noise.
 template <bool ROOT>
-__device__ __forceinline__ void hold(void* p, float* scales, int64_t at, bool live, const float (&x)[8],
-                                     const uint32_t (&r)[8], int lane) {
-  uint32_t a = 0;
+__device__ __forceinline__ void hold(void* p, float* scales, int64_t at, bool live, const Eight& x,
+                                     const uint32_t (&h)[8], int lane) {
+  float a = max_mag(x.v[0].x, x.v[0].y);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = max(a, mag(x[i]));
-  const float s = scale_of(max_over(a, 16)), inv = 1.f / s;
+  for (int i = 1; i < 4; ++i) a = max_mag(a, max_mag(x.v[i].x, x.v[i].y));
+  const float s = scale_of(max_over(__float_as_uint(a), 16)), inv = 1.f / s;
   if (!live) return;
   float c[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float y = fminf(fabsf(x[i]) * inv, kTop);
-    float d = dither(y, ROOT ? r[i] >> 16 : lower(r[i]));
-    if (ROOT && d == 0.f && y > 0.f) d = 0.001953125f;
-    c[i] = ROOT ? d : copysignf(d, x[i]);
+  for (int i = 0; i < 4; ++i) {
+    const float2 y = __fmul2_rn(x.v[i], make_float2(inv, inv));
+    const float yy[2] = {y.x, y.y};
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float z = fminf(fabsf(yy[q]), kTop);
+      if constexpr (ROOT) {
+        // upper half of the noise, four places up
+        const float d = dither(z, (h[2 * i + q] >> 12) & 0xffff0u);
+        c[2 * i + q] = fmaxf(d, z > 0.f ? 0.001953125f : 0.f);   // the smallest code, or zero for zero
+      } else {
+        c[2 * i + q] = copysignf(dither(z, lower(h[2 * i + q]) << 4), yy[q]);
+      }
+    }
   }
   *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p) + at) = code8(c, 1.f);
   if ((lane & 15) == 0) scales[at / kBlock] = s;
@@ -147,7 +176,7 @@ __global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a)
   // a state's block is whole even where the tensor ends inside it
   const bool live = at < ((it.n + kBlock - 1) & ~(int64_t)(kBlock - 1));
   const bool vec = it.flags & 2, half = it.flags & 1;
-  float p[8], g[8], m[8], v[8];
+  float p[8], g[8];
   if (half) {
     load_some(static_cast<const bf16*>(it.p) + at, vec, n, p);
     load_some(static_cast<const bf16*>(it.g) + at, vec, n, g);
@@ -155,59 +184,90 @@ __global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a)
     load_some(static_cast<const float*>(it.p) + at, vec, n, p);
     load_some(static_cast<const float*>(it.g) + at, vec, n, g);
   }
+  Eight m, v, root;
   if constexpr (EIGHT) {
-    if (live) {
-      load_codes(it.m, at, it.ms[at / kBlock], m);
-      load_codes(it.v, at, it.vs[at / kBlock], v);
+    const float sm = live ? it.ms[at / kBlock] : 0.f, sv = live ? it.vs[at / kBlock] : 0.f;
+    const int64_t in = live ? at : 0;        // lanes past the state read its start and hold nothing
+    m = load_codes(it.m, in, sm);
+    v = load_codes(it.v, in, sv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= v[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m[i] = v[i] = 0.f;
-    }
+    for (int i = 0; i < 4; ++i) v.v[i] = __fmul2_rn(v.v[i], v.v[i]);
   } else {
-    load_some(static_cast<const float*>(it.m) + at, true, n, m);
-    load_some(static_cast<const float*>(it.v) + at, true, n, v);
-  }
-  const uint32_t i0 = it.first + (uint32_t)at;
-  float root[8];
+    float t[8];
+    load_some(static_cast<const float*>(it.m) + at, true, n, t);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) m.v[i] = make_float2(t[2 * i], t[2 * i + 1]);
+    load_some(static_cast<const float*>(it.v) + at, true, n, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.v[i] = make_float2(t[2 * i], t[2 * i + 1]);
+  }
+  const uint32_t i0 = it.first + (uint32_t)at;             // a multiple of 8: i0 + i = i0 ^ i
+  const float2 b1 = make_float2(a.b1, a.b1), c1 = make_float2(a.c1, a.c1);
+  const float2 b2 = make_float2(a.b2, a.b2), c2 = make_float2(a.c2, a.c2);
+  const float ss = it.step_size, rs = it.root_scale;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
     // each operation rounded on its own, so that a restatement in elementary
     // 32-bit operations gives the same states, bit for bit
-    m[i] = __fadd_rn(__fmul_rn(a.b1, m[i]), __fmul_rn(a.c1, g[i]));
-    v[i] = __fadd_rn(__fmul_rn(a.b2, v[i]), __fmul_rn(__fmul_rn(a.c2, g[i]), g[i]));
-    root[i] = sqrtf(v[i]);
-    const float den = fmaf(root[i], it.root_scale, a.eps);
+    const float2 gg = make_float2(g[2 * i], g[2 * i + 1]);
+    m.v[i] = add_apart(__fmul2_rn(b1, m.v[i]), __fmul2_rn(c1, gg));
+    v.v[i] = add_apart(__fmul2_rn(b2, v.v[i]), __fmul2_rn(__fmul2_rn(c2, gg), gg));
+    root.v[i] = make_float2(sqrtf(v.v[i].x), sqrtf(v.v[i].y));
+    const float2 den = __ffma2_rn(root.v[i], make_float2(rs, rs), make_float2(a.eps, a.eps));
     // with 8-bit states arithmetic is the bound: the quotient may be two units of
     // its last place off, far inside a step of either format
-    const float q = EIGHT ? __fdividef(m[i], den) : m[i] / den;
-    p[i] = fmaf(-it.step_size, q, p[i] * a.keep);
+    const float2 q = EIGHT ? make_float2(__fdividef(m.v[i].x, den.x), __fdividef(m.v[i].y, den.y))
+                           : make_float2(m.v[i].x / den.x, m.v[i].y / den.y);
+    const float2 r = __ffma2_rn(make_float2(-ss, -ss), q,
+                                __fmul2_rn(make_float2(p[2 * i], p[2 * i + 1]), make_float2(a.keep, a.keep)));
+    p[2 * i] = r.x;
+    p[2 * i + 1] = r.y;
   }
   if (half) {
+    const uint32_t ik = i0 ^ (it.key + 1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t b = __float_as_uint(p[i]);
       // infinities and NaN keep their bits
-      if ((b & 0x7f800000u) != 0x7f800000u)
-        p[i] = __uint_as_float((b + lower(noise(i0 + i, it.key + 1))) & ~0xffffu);
+      p[i] = __uint_as_float(fabsf(p[i]) < __int_as_float(0x7f800000) ? b + lower(noise(ik ^ i)) : b);
     }
-    store_some(static_cast<bf16*>(it.p) + at, vec, n, p);
+    bf16* o = static_cast<bf16*>(it.p) + at;
+    if (vec && n >= 8) {                     // the upper halves are the result
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = __byte_perm(__float_as_uint(p[2 * i]), __float_as_uint(p[2 * i + 1]), 0x7632);
+      *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) o[i] = __ushort_as_bfloat16((unsigned short)(__float_as_uint(p[i]) >> 16));
+    }
   } else {
     store_some(static_cast<float*>(it.p) + at, vec, n, p);
   }
   if constexpr (EIGHT) {
-    uint32_t r[8];
+    uint32_t h[8];
+    const uint32_t ik = i0 ^ it.key;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      r[i] = noise(i0 + i, it.key);
-      if (i >= n) m[i] = root[i] = 0.f;      // past the tensor: held as zero
+    for (int i = 0; i < 8; ++i) h[i] = noise(ik ^ i);
+    if (n < 8) {                             // past the tensor: held as zero
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (2 * i >= n) m.v[i].x = root.v[i].x = 0.f;
+        if (2 * i + 1 >= n) m.v[i].y = root.v[i].y = 0.f;
+      }
     }
-    hold<false>(it.m, it.ms, at, live, m, r, lane);
-    hold<true>(it.v, it.vs, at, live, root, r, lane);
+    hold<false>(it.m, it.ms, at, live, m, h, lane);
+    hold<true>(it.v, it.vs, at, live, root, h, lane);
   } else {
-    store_some(static_cast<float*>(it.m) + at, true, n, m);
-    store_some(static_cast<float*>(it.v) + at, true, n, v);
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = m.get(i);
+    store_some(static_cast<float*>(it.m) + at, true, n, t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = v.get(i);
+    store_some(static_cast<float*>(it.v) + at, true, n, t);
   }
 }
 
@@ -278,7 +338,7 @@ extern "C" int race_adamw(const race_adamw_desc_t* desc, const race_adamw_tensor
     return RACE_ERR_INVALID;
   for (int64_t i = 0; i < count; ++i) {
     const race_adamw_tensor_t& t = tensors[i];
-    if (t.numel < 0 || t.step < 0 || (t.dtype != RACE_F32 && t.dtype != RACE_BF16)) return RACE_ERR_INVALID;
+    if (t.numel < 0 || t.step < 0 || t.first % 8 != 0 || (t.dtype != RACE_F32 && t.dtype != RACE_BF16)) return RACE_ERR_INVALID;
     if (t.numel == 0) continue;
     if (t.param == nullptr || t.grad == nullptr || t.exp_avg == nullptr || t.exp_avg_sq == nullptr)
       return RACE_ERR_INVALID;

@@ -91,7 +91,7 @@ def test_adamw_arguments(lib):
     assert f(None) == INVALID and f(d(state_bits=16)) == INVALID and f(d(beta_one=1.0)) == INVALID
     assert f(d(eps=-1.0)) == INVALID and f(d(eps=float("nan"))) == INVALID
     assert f(d(), t(numel=-1)) == INVALID and f(d(), t(param=None)) == INVALID
-    assert f(d(), t(dtype=7)) == INVALID and f(d(), t(step=-1)) == INVALID
+    assert f(d(), t(dtype=7)) == INVALID and f(d(), t(step=-1)) == INVALID and f(d(), t(first=4)) == INVALID
     assert f(d(state_bits=8)) == INVALID                      # scales are missing
     assert f(d(), t(exp_avg=ADDR + 4)) == ALIGN and f(d(), t(param=ADDR + 2)) == ALIGN
     assert lib.race_adamw(d(), None, 0, None) == 0
