@@ -13,6 +13,13 @@
 // loads a lane holds 8 consecutive columns and half a warp holds a block,
 // otherwise (odd widths or strides) lane l holds columns l, l + 32, ... and the
 // whole warp holds a block in four of its eight values.
+//
+// Rows are short (1.5 KB at 768 bfloat16 columns), so a warp that loads one, waits,
+// sums and stores keeps too few bytes on their way.  The grid is what the SMs
+// hold at once and a warp walks rows; with vector loads the next row is loaded,
+// unconverted, before the current one is summed.
+#include <atomic>
+
 #include "race_api.h"
 #include "race_lowp.cuh"
 
@@ -51,38 +58,58 @@ __device__ __forceinline__ int col_of(int s, int lane, int i) {
   return 256 * s + (VEC ? 8 * lane + i : 32 * i + lane);
 }
 
-// Vector loads need every row's base on 16 bytes; the last vector of a row may
-// be partial (width % 8), its columns then come one by one.
+// Vector loads need every row's base on 16 bytes and whole vectors (width % 8 == 0).
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_span(const T* row, int s, int lane, int width, float (&v)[8]) {
   if constexpr (VEC) {
     const int c = 256 * s + 8 * lane;
-    if (c + 8 <= width) {
+    if (c < width) {
       load8(row + c, v);
-      return;
-    }
-  }
+    } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = col_of<VEC>(s, lane, i);
-    v[i] = c < width ? to_f32(row[c]) : 0.f;
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = col_of<VEC>(s, lane, i);
+      v[i] = c < width ? to_f32(row[c]) : 0.f;
+    }
   }
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void store_span(T* row, int s, int lane, int width, const float (&v)[8]) {
   if constexpr (VEC) {
     const int c = 256 * s + 8 * lane;
-    if (c + 8 <= width) {
-      store8(row + c, v);
-      return;
+    if (c < width) store8(row + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = col_of<VEC>(s, lane, i);
+      if (c < width) row[c] = from_f32<T>(v[i]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = col_of<VEC>(s, lane, i);
-    if (c < width) row[c] = from_f32<T>(v[i]);
-  }
 }
+
+// A warp's spans of a row as they were loaded: 4 (bfloat16) or 8 registers a span.
+template <typename T, int V>
+struct Raw {
+  uint4 u[V][sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* row, int w0, int wpr, int lane, int width) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = 256 * (j * wpr + w0) + 8 * lane;
+#pragma unroll
+      for (int q = 0; q < (int)sizeof(T) / 2; ++q)
+        u[j][q] = c < width ? *reinterpret_cast<const uint4*>(row + c + q * (16 / (int)sizeof(T)))
+                            : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void get(int j, float (&v)[8]) const {
+    load8(reinterpret_cast<const T*>(&u[j][0]), v);
+  }
+};
+
 template <bool VEC>
 __device__ __forceinline__ void load_weight(const void* w, int wbf16, int s, int lane, int width,
                                             float (&v)[8]) {
@@ -120,129 +147,223 @@ template <typename T, bool VEC, int V, int WPR, bool Q>
 __global__ void __launch_bounds__(threads_of(WPR)) k_rms_fwd(const FwdArgs a) {
   __shared__ float slot[2][32];
   constexpr int RPC = threads_of(WPR) / (32 * WPR);
+  constexpr bool AHEAD = VEC && V * sizeof(T) <= 8;         // the next row waits in registers
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * RPC + warp / WPR;
   const int w0 = warp % WPR;
-  if (row >= a.rows) return;                 // whole warps only; WPR > 1 has one row per CTA
-  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-  float h[V][8];
+  const int64_t step = (int64_t)gridDim.x * RPC;
+  int64_t row = (int64_t)blockIdx.x * RPC + warp / WPR;     // the same for a row's warps
+  const T* x = static_cast<const T*>(a.x);
+  const T* res = static_cast<const T*>(a.res);
+  Raw<T, V> nx, nr;
+  if (AHEAD && row < a.rows) {
+    nx.load(x + row * a.ldx, w0, WPR, lane, a.width);
+    if (res != nullptr) nr.load(res + row * a.ldr, w0, WPR, lane, a.width);
+  }
+  int which = 0;
+  for (; row < a.rows; row += step) {
+    float h[V][8];
+    if constexpr (AHEAD) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) load_span<T, VEC>(x, j * WPR + w0, lane, a.width, h[j]);
-  if (a.res != nullptr) {
-    const T* r = static_cast<const T*>(a.res) + row * a.ldr;
-    float t[V][8];
+      for (int j = 0; j < V; ++j) {
+        nx.get(j, h[j]);
+        if (res != nullptr) {
+          float t[8];
+          nr.get(j, t);
 #pragma unroll
-    for (int j = 0; j < V; ++j) load_span<T, VEC>(r, j * WPR + w0, lane, a.width, t[j]);
+          for (int i = 0; i < 8; ++i) h[j][i] += t[i];
+        }
+      }
+      if (row + step < a.rows) {
+        nx.load(x + (row + step) * a.ldx, w0, WPR, lane, a.width);
+        if (res != nullptr) nr.load(res + (row + step) * a.ldr, w0, WPR, lane, a.width);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) load_span<T, VEC>(x + row * a.ldx, j * WPR + w0, lane, a.width, h[j]);
+      if (res != nullptr) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float t[8];
+          load_span<T, VEC>(res + row * a.ldr, j * WPR + w0, lane, a.width, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[j][i] += t[i];
+        }
+      }
+    }
+    if (res != nullptr) {
+      T* o = static_cast<T*>(a.h) + row * a.ldh;
+#pragma unroll
+      for (int j = 0; j < V; ++j) store_span<T, VEC>(o, j * WPR + w0, lane, a.width, h[j]);
+    }
+    float ss = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[j][i] += t[j][i];
-    T* o = static_cast<T*>(a.h) + row * a.ldh;
+      for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
+    ss = row_sum<WPR>(ss, slot, which);
+    which ^= 1;
+    const float rs = 1.f / sqrtf(ss / (float)a.width + a.eps);
+    if (a.rstd != nullptr && lane == 0 && w0 == 0) a.rstd[row] = rs;
 #pragma unroll
-    for (int j = 0; j < V; ++j) store_span<T, VEC>(o, j * WPR + w0, lane, a.width, h[j]);
-  }
-  float ss = 0.f;
+    for (int j = 0; j < V; ++j) {
+      const int s = j * WPR + w0;
+      if (256 * s >= a.width) break;           // the same for the whole warp
+      float w[8];
+      load_weight<VEC>(a.w, a.wbf16, s, lane, a.width, w);
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
-  ss = row_sum<WPR>(ss, slot, 0);
-  const float rs = 1.f / sqrtf(ss / (float)a.width + a.eps);
-  if (a.rstd != nullptr && lane == 0 && w0 == 0) a.rstd[row] = rs;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int s = j * WPR + w0;
-    if (256 * s >= a.width) break;           // the same for the whole warp
-    float w[8];
-    load_weight<VEC>(a.w, a.wbf16, s, lane, a.width, w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[j][i] = h[j][i] * rs * w[i];
-    if constexpr (!Q) {
-      store_span<T, VEC>(static_cast<T*>(a.y) + row * a.ldy, s, lane, a.width, h[j]);
-    } else {
-      uint8_t* c = a.codes + row * a.ldc;
-      float* sc = a.scales + row * a.sr;
-      if constexpr (VEC) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, mag(h[j][i]));
-        const float sv = scale_of(max_over(m, 16));
-        const int c0 = 256 * s + 8 * lane;
-        if (c0 < a.width) {                  // columns past the width hold zeros
-          *reinterpret_cast<uint2*>(c + c0) = code8(h[j], 1.f / sv);
-          if ((lane & 15) == 0) sc[(2 * s + (lane >> 4)) * a.sb] = sv;
-        }
+      for (int i = 0; i < 8; ++i) h[j][i] = h[j][i] * rs * w[i];
+      if constexpr (!Q) {
+        store_span<T, VEC>(static_cast<T*>(a.y) + row * a.ldy, s, lane, a.width, h[j]);
       } else {
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        uint8_t* c = a.codes + row * a.ldc;
+        float* sc = a.scales + row * a.sr;
+        if constexpr (VEC) {
           uint32_t m = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) m = max(m, mag(h[j][4 * b + i]));
-          const float sv = scale_of(max_over(m, 32));
-          const float inv = 1.f / sv;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int cc = col_of<false>(s, lane, 4 * b + i);
-            // the row's pitch is a multiple of 16: the rest of its last 16 bytes is zeroed
-            if (cc < ((a.width + 15) & ~15))
-              c[cc] = (uint8_t)code2(h[j][4 * b + i] * inv, 0.f);
+          for (int i = 0; i < 8; ++i) m = max(m, mag(h[j][i]));
+          const float sv = scale_of(max_over(m, 16));
+          const int c0 = 256 * s + 8 * lane;
+          // columns past the width hold zeros; the pitch is a multiple of 16
+          if (c0 < ((a.width + 15) & ~15)) {
+            *reinterpret_cast<uint2*>(c + c0) = code8(h[j], 1.f / sv);
+            if ((lane & 15) == 0) sc[(2 * s + (lane >> 4)) * a.sb] = sv;
           }
-          if (lane == 0 && 256 * s + 128 * b < a.width) sc[(2 * s + b) * a.sb] = sv;
+        } else {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = max(m, mag(h[j][4 * b + i]));
+            const float sv = scale_of(max_over(m, 32));
+            const float inv = 1.f / sv;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int cc = col_of<false>(s, lane, 4 * b + i);
+              // the row's pitch is a multiple of 16: the rest of its last 16 bytes is zeroed
+              if (cc < ((a.width + 15) & ~15))
+                c[cc] = (uint8_t)code2(h[j][4 * b + i] * inv, 0.f);
+            }
+            if (lane == 0 && 256 * s + 128 * b < a.width) sc[(2 * s + b) * a.sb] = sv;
+          }
         }
       }
     }
   }
 }
 
+// The CTA of the backward pass: eight warps where a warp holds a row, so that few
+// partial sums of dweight remain.
+constexpr int bwd_threads(int wpr) { return wpr == 1 ? 256 : 32 * wpr; }
+
 template <typename T, bool VEC, int V, int WPR>
-__global__ void __launch_bounds__(threads_of(WPR)) k_rms_bwd(const BwdArgs a) {
+__global__ void __launch_bounds__(bwd_threads(WPR)) k_rms_bwd(const BwdArgs a) {
   __shared__ float slot[2][32];
-  constexpr int RPC = threads_of(WPR) / (32 * WPR);
+  constexpr int RPC = bwd_threads(WPR) / (32 * WPR);
+  constexpr bool AHEAD = VEC && V * sizeof(T) <= 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int w0 = warp % WPR;
   const int64_t step = (int64_t)gridDim.x * RPC;
+  const T *dyp = static_cast<const T*>(a.dy), *hp = static_cast<const T*>(a.h), *dhp = static_cast<const T*>(a.dh);
   float dw[V][8];
 #pragma unroll
   for (int j = 0; j < V; ++j)
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[j][i] = 0.f;
   int which = 0;
-  for (int64_t row = (int64_t)blockIdx.x * RPC + warp / WPR; row < a.rows; row += step) {
-    const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
-    const T* hr = static_cast<const T*>(a.h) + row * a.ldh;
-    const float rs = a.rstd[row];
-    float g[V][8], h[V][8];
-    float dot = 0.f;
+  int64_t row = (int64_t)blockIdx.x * RPC + warp / WPR;
+  if constexpr (AHEAD) {
+    // rows stay as they were loaded and are converted where they are used, twice
+    Raw<T, V> g, h, d, ng, nh, nd;
+    float rs = 0.f, nrs = 0.f;
+    if (row < a.rows) {
+      ng.load(dyp + row * a.lddy, w0, WPR, lane, a.width);
+      nh.load(hp + row * a.ldh, w0, WPR, lane, a.width);
+      if (dhp != nullptr) nd.load(dhp + row * a.lddh, w0, WPR, lane, a.width);
+      nrs = a.rstd[row];
+    }
+    for (; row < a.rows; row += step) {
+      g = ng;
+      h = nh;
+      d = nd;
+      rs = nrs;
+      const int64_t next = row + step;
+      if (next < a.rows) {
+        ng.load(dyp + next * a.lddy, w0, WPR, lane, a.width);
+        nh.load(hp + next * a.ldh, w0, WPR, lane, a.width);
+        if (dhp != nullptr) nd.load(dhp + next * a.lddh, w0, WPR, lane, a.width);
+        nrs = a.rstd[next];
+      }
+      float dot = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) load_span<T, VEC>(dy, j * WPR + w0, lane, a.width, g[j]);
+      for (int j = 0; j < V; ++j) {
+        float w[8], gf[8], hf[8];
+        load_weight<VEC>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
+        g.get(j, gf);
+        h.get(j, hf);
 #pragma unroll
-    for (int j = 0; j < V; ++j) load_span<T, VEC>(hr, j * WPR + w0, lane, a.width, h[j]);
+        for (int i = 0; i < 8; ++i) {
+          dw[j][i] = fmaf(gf[i], hf[i] * rs, dw[j][i]);
+          dot = fmaf(gf[i] * w[i], hf[i], dot);
+        }
+      }
+      dot = row_sum<WPR>(dot, slot, which);
+      which ^= 1;
+      const float c = dot / (float)a.width * rs * rs;
+      T* dx = static_cast<T*>(a.dx) + row * a.lddx;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float w[8];
-      load_weight<VEC>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
+      for (int j = 0; j < V; ++j) {
+        float w[8], gf[8], hf[8];
+        load_weight<VEC>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
+        g.get(j, gf);
+        h.get(j, hf);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        dw[j][i] = fmaf(g[j][i], h[j][i] * rs, dw[j][i]);
-        g[j][i] *= w[i];
-        dot = fmaf(g[j][i], h[j][i], dot);
+        for (int i = 0; i < 8; ++i) gf[i] = rs * (gf[i] * w[i] - hf[i] * c);
+        if (dhp != nullptr) {
+          d.get(j, hf);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) gf[i] += hf[i];
+        }
+        store_span<T, VEC>(dx, j * WPR + w0, lane, a.width, gf);
       }
     }
-    dot = row_sum<WPR>(dot, slot, which);
-    which ^= 1;
-    const float c = dot / (float)a.width * rs * rs;
-    T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+  } else {
+    for (; row < a.rows; row += step) {
+      const T* dy = dyp + row * a.lddy;
+      const T* hr = hp + row * a.ldh;
+      const float rs = a.rstd[row];
+      float g[V][8], h[V][8];
+      float dot = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
+      for (int j = 0; j < V; ++j) load_span<T, VEC>(dy, j * WPR + w0, lane, a.width, g[j]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[j][i] = rs * (g[j][i] - h[j][i] * c);
-      if (a.dh != nullptr) {
-        float t[8];
-        load_span<T, VEC>(static_cast<const T*>(a.dh) + row * a.lddh, j * WPR + w0, lane, a.width, t);
+      for (int j = 0; j < V; ++j) load_span<T, VEC>(hr, j * WPR + w0, lane, a.width, h[j]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[j][i] += t[i];
+      for (int j = 0; j < V; ++j) {
+        float w[8];
+        load_weight<VEC>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          dw[j][i] = fmaf(g[j][i], h[j][i] * rs, dw[j][i]);
+          g[j][i] *= w[i];
+          dot = fmaf(g[j][i], h[j][i], dot);
+        }
       }
-      store_span<T, VEC>(dx, j * WPR + w0, lane, a.width, g[j]);
+      dot = row_sum<WPR>(dot, slot, which);
+      which ^= 1;
+      const float c = dot / (float)a.width * rs * rs;
+      T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[j][i] = rs * (g[j][i] - h[j][i] * c);
+        if (dhp != nullptr) {
+          float t[8];
+          load_span<T, VEC>(dhp + row * a.lddh, j * WPR + w0, lane, a.width, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[j][i] += t[i];
+        }
+        store_span<T, VEC>(dx, j * WPR + w0, lane, a.width, g[j]);
+      }
     }
   }
   float* part = a.part + (int64_t)blockIdx.x * a.width;
@@ -273,32 +394,33 @@ __global__ void __launch_bounds__(threads_of(WPR)) k_rms_bwd(const BwdArgs a) {
   }
 }
 
-// dweight[c] = sum over the CTAs' partial rows, in their order within 8 strands
-__global__ void __launch_bounds__(256) k_rms_dweight(const float* __restrict__ part, int parts,
-                                                     int width, void* __restrict__ dw, int wbf16) {
-  __shared__ float red[8][33];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5;
+// dweight[c] = sum over the CTAs' partial rows, in their order within 32 strands
+__global__ void __launch_bounds__(1024) k_rms_dweight(const float* __restrict__ part, int parts,
+                                                      int width, void* __restrict__ dw, int wbf16) {
+  __shared__ float red[32][33];
+  const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, strand = threadIdx.x >> 5;
   float t = 0.f;
   if (c < width)
-    for (int p = strand; p < parts; p += 8) t += part[(int64_t)p * width + c];
-  red[strand][threadIdx.x & 31] = t;
+    for (int p = strand; p < parts; p += 32) t += part[(int64_t)p * width + c];
+  red[strand][lane] = t;
   __syncthreads();
-  if (strand == 0 && c < width) {
-    t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t += red[i][threadIdx.x & 31];
+  // warp `strand` sums column `strand` of the 32
+  t = warp_sum(red[lane][strand]);
+  const int o = blockIdx.x * 32 + strand;
+  if (lane == 0 && o < width) {
     if (wbf16)
-      static_cast<bf16*>(dw)[c] = from_f32<bf16>(t);
+      static_cast<bf16*>(dw)[o] = from_f32<bf16>(t);
     else
-      static_cast<float*>(dw)[c] = t;
+      static_cast<float*>(dw)[o] = t;
   }
 }
 
-// CTAs of the backward pass: enough to fill the SMs, no more than there are rows
+// CTAs of the backward pass, one partial row of dweight each: at most what
+// the SMs hold at once, no more than there are rows
 int bwd_ctas(const race_norm_desc_t* d, int wpr) {
-  const int rpc = threads_of(wpr) / (32 * wpr);
+  const int rpc = bwd_threads(wpr) / (32 * wpr);
   const int64_t most = (d->rows + rpc - 1) / rpc;
-  const int64_t fill = (int64_t)api_sm_count() * (wpr == 1 ? 8 : wpr == 4 ? 8 : wpr == 16 ? 2 : 1);
+  const int64_t fill = (int64_t)api_sm_count() * (wpr == 1 ? 2 : wpr == 4 ? 4 : 1);
   return (int)(most < fill ? most : fill);
 }
 
@@ -306,18 +428,35 @@ int warps_per_row(int64_t width) {
   return width <= 1024 ? 1 : width <= 4096 ? 4 : width <= 16384 ? 16 : 32;
 }
 
+// CTAs of a kernel that the SMs hold at once
+template <typename K>
+int64_t resident(K kernel, int threads, std::atomic<int>& held) {
+  int n = held.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1) n = 1;
+    held.store(n, std::memory_order_relaxed);
+  }
+  return (int64_t)n * api_sm_count();
+}
+
+template <typename T, bool VEC, int V, int WPR, bool Q>
+void launch_fwd_as(const FwdArgs& a, cudaStream_t s) {
+  constexpr int RPC = threads_of(WPR) / (32 * WPR);
+  static std::atomic<int> held;
+  const int64_t most = (a.rows + RPC - 1) / RPC;
+  const int64_t fill = resident(&k_rms_fwd<T, VEC, V, WPR, Q>, threads_of(WPR), held);
+  k_rms_fwd<T, VEC, V, WPR, Q><<<(unsigned)(most < fill ? most : fill), threads_of(WPR), 0, s>>>(a);
+}
 template <typename T, bool VEC, int V, int WPR>
 void launch_fwd(const FwdArgs& a, cudaStream_t s) {
-  constexpr int RPC = threads_of(WPR) / (32 * WPR);
-  const unsigned grid = (unsigned)((a.rows + RPC - 1) / RPC);
   if (a.codes != nullptr)
-    k_rms_fwd<T, VEC, V, WPR, true><<<grid, threads_of(WPR), 0, s>>>(a);
+    launch_fwd_as<T, VEC, V, WPR, true>(a, s);
   else
-    k_rms_fwd<T, VEC, V, WPR, false><<<grid, threads_of(WPR), 0, s>>>(a);
+    launch_fwd_as<T, VEC, V, WPR, false>(a, s);
 }
 template <typename T, bool VEC, int V, int WPR>
 void launch_bwd(const BwdArgs& a, int grid, cudaStream_t s) {
-  k_rms_bwd<T, VEC, V, WPR><<<grid, threads_of(WPR), 0, s>>>(a);
+  k_rms_bwd<T, VEC, V, WPR><<<grid, bwd_threads(WPR), 0, s>>>(a);
 }
 
 // The spans a warp holds (V) follow from the width; the unvectorised form and
@@ -390,7 +529,7 @@ extern "C" int race_rms_norm(const race_norm_desc_t* desc, race_rows_t x, race_r
                   y8.stride_row, y8.stride_block, rstd, desc->rows, (int)desc->width, desc->eps};
   const bool f32 = desc->dtype == RACE_F32;
   const int es = f32 ? 4 : 2;
-  const bool vec = norm::aligned16(x.data, x.ld, es) && norm::aligned16(weight, 0, 1) &&
+  const bool vec = desc->width % 8 == 0 && norm::aligned16(x.data, x.ld, es) && norm::aligned16(weight, 0, 1) &&
                    (residual.data == nullptr || (norm::aligned16(residual.data, residual.ld, es) &&
                                                  norm::aligned16(h.data, h.ld, es))) &&
                    (y.data == nullptr || norm::aligned16(y.data, y.ld, es));
@@ -434,7 +573,7 @@ extern "C" int race_rms_norm_backward(const race_norm_desc_t* desc, race_rows_t 
                   static_cast<float*>(workspace), desc->rows, (int)desc->width};
   const bool f32 = desc->dtype == RACE_F32;
   const int es = f32 ? 4 : 2;
-  const bool vec = norm::aligned16(dy.data, dy.ld, es) && norm::aligned16(h.data, h.ld, es) &&
+  const bool vec = desc->width % 8 == 0 && norm::aligned16(dy.data, dy.ld, es) && norm::aligned16(h.data, h.ld, es) &&
                    norm::aligned16(dx.data, dx.ld, es) && norm::aligned16(weight, 0, 1) &&
                    (dh.data == nullptr || norm::aligned16(dh.data, dh.ld, es));
   const int wpr = norm::warps_per_row(desc->width);
@@ -444,7 +583,7 @@ extern "C" int race_rms_norm_backward(const race_norm_desc_t* desc, race_rows_t 
     norm::launch_bwd<decltype(t), decltype(ve)::value, decltype(vv)::value, decltype(ww)::value>(a, grid, stream);
   });
   api_log("rms_bwd");
-  norm::k_rms_dweight<<<(unsigned)((desc->width + 31) / 32), 256, 0, stream>>>(
+  norm::k_rms_dweight<<<(unsigned)((desc->width + 31) / 32), 1024, 0, stream>>>(
       a.part, grid, a.width, dweight, wb);
   api_log("rms_dweight");
   const cudaError_t e = cudaGetLastError();
