@@ -135,11 +135,16 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   uint32_t p;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
+  return p;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
   return v;
 }
 
@@ -162,17 +167,18 @@ __device__ __forceinline__ void report(unsigned* status, unsigned bits) {
 template <int NT>
 struct Split {
   static constexpr int A = 128 * 128, B = NT * 128, STAGE = A + B;
-  static constexpr int S = NT >= 128 ? 6 : 5;                      // stages
+  static constexpr int S = NT == 16 ? 5 : 4;                       // stages: two CTAs share an SM
   static constexpr int RED = NT * 128 * 4;                         // joined partial tile
-  static constexpr int DATA = S * STAGE > RED ? S * STAGE : RED;
-  static constexpr int SCALES = DATA;                              // [2][NT] floats
+  static constexpr int SCALES = S * STAGE;                         // [2][NT] floats
   static constexpr int BARS = SCALES + 2 * NT * 4;                 // full, empty [S]; tfull, tempty [2]; drain
   static constexpr int MISC = BARS + (2 * S + 5) * 8;              // tmem base, abort word
   static constexpr int BYTES = MISC + 16 + 1024;                   // + alignment
   static constexpr int COLS = 2 * NT < 32 ? 32 : 2 * NT;
+  static_assert(RED <= S * STAGE, "the partial tile takes the stages' place");
 };
 
 constexpr int kSplitThreads = 192;
+constexpr int kMaxCluster = 8;
 
 template <int NT, bool SQ>
 __global__ void __launch_bounds__(kSplitThreads)
@@ -211,61 +217,70 @@ __global__ void __launch_bounds__(kSplitThreads)
   __syncthreads();
   fence_after();
   const uint32_t tm = misc[0];
-
-  float acc[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j] = 0.f;
+  const uint32_t full0 = saddr(full), empty0 = saddr(empty);
+  float* red = reinterpret_cast<float*>(sm);                       // [NT][128]
 
   if (warp == 0) {
-    if (lane == 0) {
-      int i = 0;
-      for (; i < blocks; ++i) {
-        const int s = i % L::S;
-        if (i >= L::S && !bar_wait(empty + s, ((i / L::S) - 1) & 1, abort, a.polls)) break;
+    const uint32_t dst = saddr(sm);
+    int i = 0;
+    bool ok = true;
+    for (; i < blocks; ++i) {
+      const int s = i % L::S;
+      if (i >= L::S) ok = wait(empty0 + 8 * s, ((i / L::S) - 1) & 1, abort, a.polls);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (elect()) {
         bar_expect_tx(full + s, L::STAGE);
-        const uint32_t dst = saddr(sm) + s * L::STAGE;
-        tma2(dst, &mapw, (k0 + i) * 128, (int)n0, saddr(full + s));
-        tma2(dst + L::A, &mapx, (k0 + i) * 128, (int)m0, saddr(full + s));
+        tma2(dst + s * L::STAGE, &mapw, (k0 + i) * 128, (int)n0, full0 + 8 * s);
+        tma2(dst + s * L::STAGE + L::A, &mapx, (k0 + i) * 128, (int)m0, full0 + 8 * s);
       }
-      if (i < blocks) {                                            // gave up: copies in flight land first
-        for (int j = i > L::S ? i - L::S : 0; j < i; ++j)
-          if (!bar_wait(full + j % L::S, (j / L::S) & 1)) report(a.status, t5::kErrStuck);
-      } else {                                                     // the last commits have arrived
-        for (int j = i > L::S ? i - L::S : 0; j < i; ++j)
-          if (!bar_wait(empty + j % L::S, (j / L::S) & 1, abort, a.polls)) break;
-      }
+      __syncwarp();
+    }
+    const int from = i > L::S ? i - L::S : 0;
+    if (i < blocks) {                                              // gave up: copies in flight land first
+      for (int j = from; j < i; ++j)
+        if (!bar_wait(full + j % L::S, (j / L::S) & 1) && lane == 0) report(a.status, t5::kErrStuck);
+    } else {                                                       // the last commits have arrived
+      for (int j = from; j < i && ok; ++j) ok = wait(empty0 + 8 * (j % L::S), (j / L::S) & 1, abort, a.polls);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int i = 0;
-      for (; i < blocks; ++i) {
-        const int s = i % L::S, b = i & 1;
-        if (i >= 2 && !bar_wait(tempty + b, ((i >> 1) - 1) & 1, abort, a.polls)) break;
-        if (!bar_wait(full + s, (i / L::S) & 1, abort, a.polls)) break;
-        fence_after();
-        const uint8_t* st = sm + s * L::STAGE;
+    const uint64_t da = t5::desc_sw128(sm, 0), db = t5::desc_sw128(sm + L::A, 0);
+    const uint32_t tempty0 = saddr(tempty);
+    int i = 0;
+    for (; i < blocks; ++i) {
+      const int s = i % L::S, b = i & 1;
+      const bool ok = wait(full0 + 8 * s, (i / L::S) & 1, abort, a.polls) &&
+                      (i < 2 || wait(tempty0 + 8 * b, ((i >> 1) - 1) & 1, abort, a.polls));
+      if (!__all_sync(0xffffffffu, ok)) break;
+      fence_after();
+      if (elect()) {
+        const uint64_t at = (uint64_t)(s * (L::STAGE >> 4));
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
-          mma8(tm + b * NT, t5::desc_sw128(st, ks), t5::desc_sw128(st + L::A, ks), idesc8<128, NT>(),
-               ks > 0);
-        t5::commit(empty + s);
+          mma8(tm + b * NT, da + at + 2 * ks, db + at + 2 * ks, idesc8<128, NT>(), ks > 0);
         t5::commit(tfull + b);
+        t5::commit(empty + s);
       }
-      if (i < blocks) {
-        t5::commit(drain);
-        if (!bar_wait(drain, 0)) report(a.status, t5::kErrStuck);
-      }
+      __syncwarp();
+    }
+    if (i < blocks) {
+      if (elect()) t5::commit(drain);
+      __syncwarp();
+      if (!bar_wait(drain, 0) && lane == 0) report(a.status, t5::kErrStuck);
     }
   } else {
     // row of the tile (weight row) = tensor-memory lane; columns = tokens
     const int quarter = warp & 3, row = 32 * quarter + lane, pt = tid - 64;
+    const uint32_t lanes = tm + ((uint32_t)(32 * quarter) << 16), tf = saddr(tfull);
     float* sx = reinterpret_cast<float*>(sm + L::SCALES);
     const int64_t wr = SQ ? blockIdx.y : (n0 + row < a.n ? n0 + row : a.n - 1);
     const float* sw = a.sb + wr * a.sbr + k0 * a.sbb;
     const bool tok = pt < NT && m0 + pt < a.m;
     const float* sxg = a.sa + (tok ? m0 + pt : 0) * a.sar + k0 * a.sab;
-    float nx = tok && blocks > 0 ? __ldg(sxg) : 0.f;
-    float nw = blocks > 0 ? __ldg(sw) : 0.f;
+    float nx = tok ? __ldg(sxg) : 0.f;
+    float nw = __ldg(sw);
+    float acc[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j] = 0.f;
     for (int i = 0; i < blocks; ++i) {
       const int b = i & 1;
       const float w = nw;
@@ -276,69 +291,82 @@ __global__ void __launch_bounds__(kSplitThreads)
         if (tok) nx = __ldg(sxg + (i + 1) * a.sab);
         nw = __ldg(sw + (i + 1) * a.sbb);
       }
-      // a thread that gives up leaves through the same barriers as the rest
-      const bool ok = bar_wait(tfull + b, (i >> 1) & 1, abort, a.polls);
-      if (__any_sync(0xffffffffu, !ok)) continue;
+      // a wait that ran out leaves garbage here, which is not stored
+      wait(tf + 8 * b, (i >> 1) & 1, abort, a.polls);
+      __syncwarp();
       fence_after();
-      constexpr int G = NT < 32 ? NT : 32;
 #pragma unroll
-      for (int c = 0; c < NT; c += G) {
-        float v[G];
-#pragma unroll
-        for (int q = 0; q < G; q += 16) {
-          float (&vq)[16] = *reinterpret_cast<float (*)[16]>(&v[q]);
-          t5::tld16(tm + ((uint32_t)(32 * quarter) << 16) + b * NT + c + q, vq);
-        }
+      for (int c = 0; c < NT; c += 16) {
+        float v[16];
+        t5::tld16(lanes + b * NT + c, v);
         t5::tld_wait();
-        if (c + G == NT) {
+        if (c + 16 == NT) {
           fence_before();
           __syncwarp();
           if (lane == 0) bar_arrive(tempty + b);
         }
 #pragma unroll
-        for (int q = 0; q < G; q += 4) {
-          const float4 s4 = *reinterpret_cast<const float4*>(sxb + c + q);
-          acc[c + q] = fmaf(s4.x * w, v[q], acc[c + q]);
-          acc[c + q + 1] = fmaf(s4.y * w, v[q + 1], acc[c + q + 1]);
-          acc[c + q + 2] = fmaf(s4.z * w, v[q + 2], acc[c + q + 2]);
-          acc[c + q + 3] = fmaf(s4.w * w, v[q + 3], acc[c + q + 3]);
+        for (int q = 0; q < 16; q += 2) {
+          const float2 s2 = __fmul2_rn(*reinterpret_cast<const float2*>(sxb + c + q), make_float2(w, w));
+          const float2 r = __ffma2_rn(s2, make_float2(v[q], v[q + 1]), make_float2(acc[c + q], acc[c + q + 1]));
+          acc[c + q] = r.x;
+          acc[c + q + 1] = r.y;
         }
       }
     }
+    // every copy into the stages has been used: they now hold the partial tile
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < NT; ++j) red[j * 128 + row] = acc[j];
   }
   __syncthreads();
   const bool failed = *abort != 0;
   if (failed && tid == 0) report(a.status, t5::kErrTimeout);
   if (warp == 1) t5::tmem_free<L::COLS>(tm);
-
-  const int quarter = warp & 3, row = 32 * quarter + lane;
-  const int64_t col = n0 + row;
-  if (C == 1) {
-    if (warp >= 2 && col < a.n && !failed) {
+  if (C > 1) cluster_sync();
+  // The ranks share the tile's tokens; a thread joins four weight rows of one,
+  // all partials on their way at once, summed in the order of the ranks.
+  if (!failed) {
+    const int q = tid & 31;
+    const int64_t col = n0 + 4 * q;
+    const bool vec = a.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && col + 4 <= a.n;
+    const int64_t left = a.m - m0;
+    const int rows = left < NT ? (int)left : NT;
+    for (int j = rank + C * (tid >> 5); j < rows; j += C * (kSplitThreads / 32)) {
+      const uint32_t at = saddr(red + j * 128 + 4 * q);
+      float4 t;
+      if (C == 1) {
+        t = *reinterpret_cast<const float4*>(red + j * 128 + 4 * q);
+      } else {
+        float4 v[kMaxCluster];
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        if (m0 + j < a.m) put(a, m0 + j, col, acc[j]);
-    }
-    return;
-  }
-  // every copy into the stages has been used: they now hold the partial tile
-  float* red = reinterpret_cast<float*>(sm);
-  if (warp >= 2) {
+        for (int r = 0; r < kMaxCluster; ++r)
+          if (r < C) v[r] = ld_cluster4(map_rank(at, r));
+        t = v[0];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) red[j * 128 + row] = acc[j];
-  }
-  __syncwarp();
-  cluster_sync();
-  if (warp >= 2 && !failed) {
-    for (int j = rank; j < NT; j += C) {
-      if (m0 + j >= a.m) break;
-      float t = 0.f;
-      for (int r = 0; r < C; ++r) t += ld_cluster(saddr(red + j * 128 + row), r);
-      if (col < a.n) put(a, m0 + j, col, t);
+        for (int r = 1; r < kMaxCluster; ++r)
+          if (r < C) {
+            t.x += v[r].x; t.y += v[r].y; t.z += v[r].z; t.w += v[r].w;
+          }
+      }
+      if (vec && a.ybf16) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(t.x, t.y), hi = __floats2bfloat162_rn(t.z, t.w);
+        *reinterpret_cast<uint2*>(static_cast<bf16*>(a.y) + (m0 + j) * a.ldy + col) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      } else if (vec) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.y) + (m0 + j) * a.ldy + col) = t;
+      } else {
+        const float e[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          if (col + z < a.n) put(a, m0 + j, col + z, e[z]);
+      }
     }
   }
-  __syncwarp();
-  cluster_sync();                                                  // peers may still be reading
+  if (C > 1) {
+    __syncwarp();
+    cluster_sync();                                                // peers may still be reading
+  }
 }
 
 // Opts a kernel in to its shared memory, once on each device.
@@ -403,11 +431,6 @@ struct Pair {
   static_assert(BYTES <= 232448, "227 KB of shared memory");
 };
 
-__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
-  uint32_t p;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
-  return p;
-}
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -794,7 +817,7 @@ struct Plan {
 Plan plan_of(int64_t m, int64_t n, int64_t k) {
   Plan p{};
   const int64_t kb = (k + 127) / 128, sms = api_sm_count();
-  p.nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+  p.nt = m <= 16 ? 16 : m <= 32 ? 32 : 64;
   p.c = 1;
   const int64_t tiles = ((n + 127) / 128) * ((m + p.nt - 1) / p.nt);
   while (p.c < 8 && tiles * p.c * 2 <= 2 * sms && p.c * 2 <= kb) p.c *= 2;
@@ -897,7 +920,6 @@ extern "C" int race_scaled_matmul(const race_matmul_desc_t* desc, race_blocks_t 
   switch (plan.nt) {
     case 16: return mm::launch_split<16>(g, mb, ma, square, plan.c, stream);
     case 32: return mm::launch_split<32>(g, mb, ma, square, plan.c, stream);
-    case 64: return mm::launch_split<64>(g, mb, ma, square, plan.c, stream);
-    default: return mm::launch_split<128>(g, mb, ma, square, plan.c, stream);
+    default: return mm::launch_split<64>(g, mb, ma, square, plan.c, stream);
   }
 }
