@@ -806,8 +806,17 @@ int launch_pair(const PairArgs& p, const CUtensorMap& ma, const CUtensorMap& mb,
   return e == cudaSuccess ? RACE_OK : api_cuda_fail(e);
 }
 
-// How a product is cut.  Measured on 148 SMs, in the time of one block on a
-// pair (512 cycles of its tensor core): see the comment at each figure.
+// How a product is cut: the cheaper of the two kernels by their measured times
+// (148 SMs, operands in L2; kb = blocks of the contraction).
+//   k_mm_split: 4 us and 0.39 us a block while every tile has an SM; from about 288
+//     tiles of 64 tokens on, 330 tile-blocks a us (1024 x 2304 x 768 8.1 us, 2048 14.0).
+//     Joining a cluster's ranks costs 1.6 us for 64 tokens and 0.4 us for 16 (and
+//     an SM for each rank: at two ranks an SM 256 x 2304 x 768 takes 11.0 us in place
+//     of 6.3), each rank taken off saves its blocks: 64 x 4096 x 4096 16.5, 12.0,
+//     8.6, 9.8 us for 1, 2, 4, 8 ranks, 16 x 8192 x 8192 25.8, 15.5, 11.7, 16.0.
+//   k_mm_pair: 6.4 us, and 0.45 us a block and 1 us a tile for every round of the 74
+//     pairs (2048 x 2304 x 768 9.2 us, 1024 x 4096 x 4096 20.2); a contraction cut in
+//     s adds 2.5 us and the partial results' way at 5 TB/s.
 struct Plan {
   bool pair;
   int nt, c;               // k_mm_split: token columns of a tile, CTAs of a cluster
@@ -816,31 +825,37 @@ struct Plan {
 
 Plan plan_of(int64_t m, int64_t n, int64_t k) {
   Plan p{};
-  const int64_t kb = (k + 127) / 128, sms = api_sm_count();
+  const int64_t kb = (k + 127) / 128, sms = api_sm_count(), pairs = sms / 2;
   p.nt = m <= 16 ? 16 : m <= 32 ? 32 : 64;
-  p.c = 1;
+  const double join = p.nt == 64 ? 1.6 : 0.4;
   const int64_t tiles = ((n + 127) / 128) * ((m + p.nt - 1) / p.nt);
-  while (p.c < 8 && tiles * p.c * 2 <= 2 * sms && p.c * 2 <= kb) p.c *= 2;
+  const int64_t room = p.nt == 64 ? sms : 2 * sms;
+  double split = 1e30, pair = 1e30;
+  for (int c = 1; c <= kMaxCluster && 2 * c <= 3 * kb; c *= 2) {
+    if (c > 1 && tiles * c > room) break;
+    const double each = 4.0 + 0.39 * (double)((kb + c - 1) / c) + (c > 1 ? join : 0.0) + (c > 4 ? join : 0.0);
+    const double all = 2.0 + (double)(tiles * kb) / 330.0 * (p.nt == 64 ? 1.0 : 0.5);
+    const double t = each > all ? each : all;
+    if (t < split) {
+      split = t;
+      p.c = c;
+    }
+  }
   p.tiles_m = (int)((m + 255) / 256);
   p.tiles_n = (int)((n + 255) / 256);
   p.splits = 1;
-  const int64_t big = (int64_t)p.tiles_m * p.tiles_n, pairs = sms / 2;
-  // a whole round of pairs, or a contraction long enough to be cut into one
-  p.pair = m > 128 && n > 128 && (big >= pairs || big * (kb / 16) >= pairs);
-  if (p.pair && big < 4 * pairs) {
-    // rounds of the pairs times blocks of an item, plus the partial results'
-    // way to memory and back
-    double best = 1e30;
-    for (int s = 1; s <= 32 && s <= kb; ++s) {
+  const int64_t big = (int64_t)p.tiles_m * p.tiles_n;
+  if (m > 128 && n > 128)
+    for (int s = 1; s <= 32 && s <= kb && (s == 1 || big < 4 * pairs); ++s) {
       const double rounds = (double)((big * s + pairs - 1) / pairs);
-      const double cost = rounds * ((double)((kb + s - 1) / s) + 3.0) +
-                          (s > 1 ? 8.0 + s * (double)(m * n) * 1.6e-6 * 4 : 0.0);
-      if (cost < best) {
-        best = cost;
+      const double t = 6.4 + rounds * (0.45 * (double)((kb + s - 1) / s) + 1.0) +
+                       (s > 1 ? 2.5 + s * (double)(m * n) * 4 / 5e6 : 0.0);
+      if (t < pair) {
+        pair = t;
         p.splits = s;
       }
     }
-  }
+  p.pair = pair < split;
   return p;
 }
 
