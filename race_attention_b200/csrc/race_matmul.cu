@@ -412,6 +412,8 @@ struct PairArgs {
   Args a;
   int tiles_m, tiles_n;    // 256 x 256 tiles
   int splits;              // of the contraction
+  uint32_t group_mul;      // x / (kGroup tiles_n) = x group_mul >> 32 >> group_shift
+  int group_shift;
   float* part;             // splits > 1: [split][m][n] partial results
   int store;               // 1: results leave by TMA (map y), 0: element by element
 };
@@ -451,9 +453,8 @@ __device__ __forceinline__ void tma2_store(const CUtensorMap* map, int c0, int c
                "r"(c0), "r"(c1), "r"(src)
                : "memory");
 }
-template <int N>
 __device__ __forceinline__ void store_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 __device__ __forceinline__ void mma8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
   asm volatile(
@@ -475,17 +476,27 @@ __device__ __forceinline__ void arrive_at(uint32_t bar) {
 struct Item {
   int m, n, k0, k1, split;
 };
+// blocks [k0, k1) of item i's contraction; whole contractions need no division
+__device__ __forceinline__ void range_of(const PairArgs& p, int i, int& k0, int& k1) {
+  if (p.splits == 1) {
+    k0 = 0;
+    k1 = p.a.kb;
+  } else {
+    const int split = i / (p.tiles_m * p.tiles_n);
+    k0 = (int)((int64_t)p.a.kb * split / p.splits);
+    k1 = (int)((int64_t)p.a.kb * (split + 1) / p.splits);
+  }
+}
 __device__ __forceinline__ Item item_of(const PairArgs& p, int i) {
   const int tiles = p.tiles_m * p.tiles_n;
   Item t;
-  t.split = i / tiles;
+  t.split = p.splits == 1 ? 0 : i / tiles;
   const int r = i - t.split * tiles;
-  const int g = r / (kGroup * p.tiles_n), first = g * kGroup;
+  const int g = (int)((((uint64_t)r * p.group_mul) >> 32) >> p.group_shift), first = g * kGroup;
   const int rows = min(kGroup, p.tiles_m - first), l = r - first * p.tiles_n;
-  t.m = first + l % rows;
-  t.n = l / rows;
-  t.k0 = (int)((int64_t)p.a.kb * t.split / p.splits);
-  t.k1 = (int)((int64_t)p.a.kb * (t.split + 1) / p.splits);
+  t.n = rows == kGroup ? l / kGroup : l / rows;
+  t.m = first + l - t.n * rows;
+  range_of(p, i, t.k0, t.k1);
   return t;
 }
 
@@ -570,8 +581,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const uint32_t tempty0 = saddr(tempty);
       int it = 0;
       for (int i = cluster; ok && i < items; i += clusters) {
-        const Item t = item_of(p, i);
-        for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
+        int k0, k1;
+        range_of(p, i, k0, k1);
+        for (int kb = k0; kb < k1; ++kb, ++it) {
           const int b = it & 1;
           ok = wait(full0 + 8 * s, ph, abort, a.polls) &&
                (it < 2 || wait(tempty0 + 8 * b, ((it >> 1) - 1) & 1, abort, a.polls));
@@ -608,18 +620,31 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     uint8_t* box = sm + L::OUT + (warp - 4) * 8192;
     float* sbs = reinterpret_cast<float*>(sm + L::SCALES) + 128 * part;
     int it = 0;
+    // A tile's scales: this thread's row of a, and of b the 128 columns' block
+    // (square) or column `row`.  The next tile and its first scales are found during
+    // this one's first block: in the epilogue they would stand in the way.
+    const float *sa = nullptr, *sb = nullptr, *nsa = nullptr, *nsb = nullptr;
+    float na = 0.f, nb = 0.f, fa = 0.f, fb = 0.f;
+    Item next = item_of(p, cluster);
+    const auto fetch = [&]() {
+      const int64_t mr = (int64_t)next.m * 256 + rank * 128 + row, n0 = (int64_t)next.n * 256 + 128 * part;
+      nsa = a.sa + (mr < a.m ? mr : a.m - 1) * a.sar + next.k0 * a.sab;
+      nsb = a.sb + (SQ ? min(n0, a.n - 1) / 128 : min(n0 + row, a.n - 1)) * a.sbr + next.k0 * a.sbb;
+      fa = __ldg(nsa);
+      fb = __ldg(nsb);
+    };
+    if (cluster < items) fetch();
     for (int i = cluster; i < items; i += clusters) {
-      const Item t = item_of(p, i);
+      const Item t = next;
       const int64_t mr = (int64_t)t.m * 256 + rank * 128 + row;    // this thread's row of the result
-      const int64_t n0 = (int64_t)t.n * 256 + 128 * part;           // its first column
-      const float* sa = a.sa + (mr < a.m ? mr : a.m - 1) * a.sar;
-      // square: one scale for the 128 columns; else thread `row` fetches that of column `row`
-      const int64_t br = SQ ? min(n0, a.n - 1) / 128 : min(n0 + row, a.n - 1);
-      const float* sb = a.sb + br * a.sbr;
+      const int64_t n0 = (int64_t)t.n * 256 + 128 * part;          // its first column
+      sa = nsa;
+      sb = nsb;
+      na = fa;
+      nb = fb;
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
-      float na = __ldg(sa + t.k0 * a.sab), nb = __ldg(sb + t.k0 * a.sbb);
       for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
         const int b = it & 1;
         const float ca = na, cb = nb;
@@ -629,8 +654,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");   // the four warps of these columns
         }
         if (kb + 1 < t.k1) {
-          na = __ldg(sa + (kb + 1) * a.sab);
-          nb = __ldg(sb + (kb + 1) * a.sbb);
+          sa += a.sab;
+          sb += a.sbb;
+          na = __ldg(sa);
+          nb = __ldg(sb);
+        }
+        if (kb == t.k0 && i + clusters < items) {
+          next = item_of(p, i + clusters);
+          fetch();
         }
         // a wait that ran out leaves garbage here, which is not stored
         wait(tf + 8 * b, (it >> 1) & 1, abort, a.polls);
@@ -681,40 +712,48 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
         }
       } else if (p.store) {
-        // 128 bytes of 32 rows at a time, 16-byte chunk c of row r at c ^ (r % 8)
-        const int es = a.ybf16 ? 2 : 4;
+        // Two boxes of 32 rows x 128 bytes at a time (bfloat16: all 128 columns),
+        // 16-byte chunk c of row r at c ^ (r % 8).
         const int r0 = (int)(mr - lane);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if (a.ybf16 && g >= 2) break;
-          uint8_t* o = box + 4096 * (g & 1);
-          if (lane == 0) store_wait_read<1>();                     // the box's last store has read it
+        if (a.ybf16) {
+          if (lane == 0) store_wait_read();                        // the last tile's stores have read the boxes
           __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint4 u;
-            if (a.ybf16) {
-              uint32_t w[4];
+          for (int c = 0; c < 16; ++c) {
+            uint32_t w[4];
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const int j = (g & 1) * 64 + 8 * c + 2 * q;
-                const __nv_bfloat162 h = __floats2bfloat162_rn(acc[j], acc[j + 1]);
-                w[q] = *reinterpret_cast<const uint32_t*>(&h);
-              }
-              u = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
-              const int j = g * 32 + 4 * c;
-              u = make_uint4(__float_as_uint(acc[j]), __float_as_uint(acc[j + 1]),
-                             __float_as_uint(acc[j + 2]), __float_as_uint(acc[j + 3]));
+            for (int q = 0; q < 4; ++q) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(acc[8 * c + 2 * q], acc[8 * c + 2 * q + 1]);
+              w[q] = *reinterpret_cast<const uint32_t*>(&h);
             }
-            *reinterpret_cast<uint4*>(o + lane * 128 + ((c ^ (lane & 7)) << 4)) = u;
+            *reinterpret_cast<uint4*>(box + (c >> 3) * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
           }
           t5::fence_async_smem();
           __syncwarp();
-          const int64_t col = n0 + g * (128 / es);
-          if (lane == 0) {
-            if (col < a.n && r0 < a.m) tma2_store(&mapy, (int)(col * es), r0, saddr(o));
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // one group a box, stored or not
+          if (lane == 0 && r0 < a.m) {
+            if (n0 < a.n) tma2_store(&mapy, (int)n0 * 2, r0, saddr(box));
+            if (n0 + 64 < a.n) tma2_store(&mapy, (int)n0 * 2 + 128, r0, saddr(box) + 4096);
+          }
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        } else {
+#pragma unroll
+          for (int g = 0; g < 4; g += 2) {
+            if (lane == 0) store_wait_read();
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              *reinterpret_cast<float4*>(box + (c >> 3) * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) =
+                  make_float4(acc[32 * g + 4 * c], acc[32 * g + 4 * c + 1], acc[32 * g + 4 * c + 2],
+                              acc[32 * g + 4 * c + 3]);
+            t5::fence_async_smem();
+            __syncwarp();
+            const int64_t col = n0 + 32 * g;
+            if (lane == 0 && r0 < a.m) {
+              if (col < a.n) tma2_store(&mapy, (int)col * 4, r0, saddr(box));
+              if (col + 32 < a.n) tma2_store(&mapy, (int)col * 4 + 128, r0, saddr(box) + 4096);
+            }
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         }
       } else if (mr < a.m) {
@@ -723,7 +762,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (n0 + j < a.n) put(a, mr, n0 + j, acc[j]);
       }
     }
-    if (lane == 0) store_wait_read<0>();
+    if (lane == 0) store_wait_read();
   }
   __syncthreads();
   cluster_sync();
@@ -920,7 +959,13 @@ extern "C" int race_scaled_matmul(const race_matmul_desc_t* desc, race_blocks_t 
         !(store ? api_encode_bytes(&my, result.data, desc->m, desc->n * es, result.ld * es, 32)
                 : api_encode_bytes(&my, a.codes, desc->m, desc->k, a.ld, 32)))
       return RACE_ERR_UNSUPPORTED;
-    const mm::PairArgs p{g, plan.tiles_m, plan.tiles_n, plan.splits, static_cast<float*>(workspace), store};
+    // x / d for 0 <= x < 2^31: with 2^s < d <= 2^(s + 1), mul = ceil(2^(32 + s) / d) < 2^32
+    const uint64_t d = (uint64_t)mm::kGroup * plan.tiles_n;
+    int shift = 0;
+    while ((uint64_t(2) << shift) < d) ++shift;
+    const uint32_t mul = (uint32_t)(((uint64_t(1) << (32 + shift)) + d - 1) / d);
+    const mm::PairArgs p{g, plan.tiles_m, plan.tiles_n, plan.splits, mul, shift,
+                         static_cast<float*>(workspace), store};
     return square ? mm::launch_pair<true>(p, ma, mb, my, stream)
                   : mm::launch_pair<false>(p, ma, mb, my, stream);
   }
