@@ -69,12 +69,21 @@ __device__ __forceinline__ uint32_t lower(uint32_t h) { return (h ^ (h >> 16)) &
 
 // y in [0, 448] up or down to the 8-bit format, r of 65536ths deciding (r20 = 16 r):
 // below 2^-6 the format's steps are even, as they are for every number of the
-// binade that adding 2^-6 moves y to.
+// binade that adding 2^-6 moves y to.  Whether y is below comes from a saturated
+// product, 0 or 1 (2^-6 - y is 2^-30 at least if it is above zero): the logic units
+// are the bound here, the multipliers are not.  A y that rounding put one place
+// above 448 still gives 448.
 __device__ __forceinline__ float dither(float y, uint32_t r20) {
-  const bool low = y < 0.015625f;
-  const float z = low ? y + 0.015625f : y;
-  const float t = __uint_as_float((__float_as_uint(z) + r20) & ~0xfffffu);
-  return low ? t - 0.015625f : t;
+  const float low = __saturatef(fmaf(y, -0x1p40f, 0x1p34f));
+  const uint32_t b = __float_as_uint(fmaf(low, 0.015625f, y)) + r20;
+  return fmaf(low, -0.015625f, __uint_as_float(b & ~0xfffffu));
+}
+
+// to two units of the last place, infinite for zero
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // the larger magnitude, NaN if one is
@@ -142,17 +151,16 @@ __device__ __forceinline__ void hold(void* p, float* scales, int64_t at, bool li
   float c[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 y = __fmul2_rn(x.v[i], make_float2(inv, inv));
-    const float yy[2] = {y.x, y.y};
+    const float yy[2] = {x.v[i].x * inv, x.v[i].y * inv};
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const float z = fminf(fabsf(yy[q]), kTop);
+      const uint32_t r = h[2 * i + q];
       if constexpr (ROOT) {
-        // upper half of the noise, four places up
-        const float d = dither(z, (h[2 * i + q] >> 12) & 0xffff0u);
-        c[2 * i + q] = fmaxf(d, z > 0.f ? 0.001953125f : 0.f);   // the smallest code, or zero for zero
+        // upper half of the noise, four places up; above zero at least the smallest code
+        const float d = dither(yy[q], (r >> 12) & 0xffff0u);
+        c[2 * i + q] = fmaxf(d, fminf(yy[q] * 1e30f, 0.001953125f));
       } else {
-        c[2 * i + q] = copysignf(dither(z, lower(h[2 * i + q]) << 4), yy[q]);
+        c[2 * i + q] = copysignf(dither(fabsf(yy[q]), lower(r) << 4), yy[q]);
       }
     }
   }
@@ -171,11 +179,11 @@ __global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a)
   const Item& it = a.item[lo];
   const int64_t c0 = (int64_t)(chunk - (lo > 0 ? a.end[lo - 1] : 0)) * CHUNK;
   const int lane = threadIdx.x & 31;
+  const bool vec = it.flags & 2, half = it.flags & 1;
   const int64_t at = c0 + 8 * (int64_t)threadIdx.x;
   const int n = (int)min((int64_t)8, max((int64_t)0, it.n - at));    // elements of this thread
   // a state's block is whole even where the tensor ends inside it
   const bool live = at < ((it.n + kBlock - 1) & ~(int64_t)(kBlock - 1));
-  const bool vec = it.flags & 2, half = it.flags & 1;
   float p[8], g[8];
   if (half) {
     load_some(static_cast<const bf16*>(it.p) + at, vec, n, p);
@@ -216,7 +224,7 @@ __global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a)
     const float2 den = __ffma2_rn(root.v[i], make_float2(rs, rs), make_float2(a.eps, a.eps));
     // with 8-bit states arithmetic is the bound: the quotient may be two units of
     // its last place off, far inside a step of either format
-    const float2 q = EIGHT ? make_float2(__fdividef(m.v[i].x, den.x), __fdividef(m.v[i].y, den.y))
+    const float2 q = EIGHT ? __fmul2_rn(m.v[i], make_float2(reciprocal(den.x), reciprocal(den.y)))
                            : make_float2(m.v[i].x / den.x, m.v[i].y / den.y);
     const float2 r = __ffma2_rn(make_float2(-ss, -ss), q,
                                 __fmul2_rn(make_float2(p[2 * i], p[2 * i + 1]), make_float2(a.keep, a.keep)));
@@ -225,11 +233,18 @@ __global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a)
   }
   if (half) {
     const uint32_t ik = i0 ^ (it.key + 1);
+    float zero = 0.f;                        // NaN as soon as one of the eight is not finite
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t b = __float_as_uint(p[i]);
-      // infinities and NaN keep their bits
-      p[i] = __uint_as_float(fabsf(p[i]) < __int_as_float(0x7f800000) ? b + lower(noise(ik ^ i)) : b);
+    for (int i = 0; i < 8; ++i) zero = fmaf(p[i], 0.f, zero);
+    if (zero == 0.f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        p[i] = __uint_as_float(__float_as_uint(p[i]) + lower(noise(ik ^ i)));
+    } else {                                 // infinities and NaN keep their bits
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (fabsf(p[i]) < __int_as_float(0x7f800000))
+          p[i] = __uint_as_float(__float_as_uint(p[i]) + lower(noise(ik ^ i)));
     }
     bf16* o = static_cast<bf16*>(it.p) + at;
     if (vec && n >= 8) {                     // the upper halves are the result
