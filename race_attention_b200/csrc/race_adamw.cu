@@ -23,6 +23,7 @@
 // The noise is a hash of the element's index, the seed and t, two odd
 // multipliers (2^32 over the golden ratio; the fraction of sqrt(2)) between shifts.
 #include <cmath>
+#include <type_traits>
 
 #include "race_api.h"
 #include "race_lowp.cuh"
@@ -33,7 +34,8 @@ namespace adamw {
 using namespace lowp;
 
 constexpr int NT = 256;
-constexpr int CHUNK = 8 * NT;
+constexpr int kChunk = 8 * NT;         // elements of a CTA at a time
+constexpr int kRounds = 4;             // of the 8-bit form with bfloat16 parameters
 constexpr uint32_t kGolden = 0x9E3779B1u, kRootTwo = 0x6A09E667u;
 
 struct Item {
@@ -124,10 +126,8 @@ __device__ __forceinline__ float2 add_apart(float2 a, float2 b) {
   return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y));
 }
 
-// eight codes of a state's block (states start on 128-element boundaries, so
-// whole words are always inside them)
-__device__ __forceinline__ Eight load_codes(const void* p, int64_t at, float s) {
-  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p) + at);
+// eight codes as values
+__device__ __forceinline__ Eight decode(uint2 u, float s) {
   Eight e;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -168,23 +168,79 @@ __device__ __forceinline__ void hold(void* p, float* scales, int64_t at, bool li
   if ((lane & 15) == 0) scales[at / kBlock] = s;
 }
 
-template <int N, bool EIGHT>
-__global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a) {
+// The tensor that chunk `chunk` belongs to: bisection over the running counts.
+template <int N>
+__device__ __forceinline__ int tensor_of(const Args<N>& a, int chunk) {
   int lo = 0, hi = a.count - 1;
-  const int chunk = blockIdx.x;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (chunk < a.end[mid]) hi = mid; else lo = mid + 1;
   }
+  return lo;
+}
+
+// m, v, the root and the parameters after the step; each operation of the states
+// is rounded on its own, so that a restatement in elementary 32-bit operations
+// gives the same states, bit for bit.  FAST: with 8-bit states arithmetic is the
+// bound; the quotient may be two units of its last place off, far inside a step
+// of either format.
+template <bool FAST, int N>
+__device__ __forceinline__ void update(const Args<N>& a, float ss, float rs, float (&p)[8], const float (&g)[8],
+                                       Eight& m, Eight& v, Eight& root) {
+  const float2 b1 = make_float2(a.b1, a.b1), c1 = make_float2(a.c1, a.c1);
+  const float2 b2 = make_float2(a.b2, a.b2), c2 = make_float2(a.c2, a.c2);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 gg = make_float2(g[2 * i], g[2 * i + 1]);
+    m.v[i] = add_apart(__fmul2_rn(b1, m.v[i]), __fmul2_rn(c1, gg));
+    v.v[i] = add_apart(__fmul2_rn(b2, v.v[i]), __fmul2_rn(__fmul2_rn(c2, gg), gg));
+    root.v[i] = make_float2(sqrtf(v.v[i].x), sqrtf(v.v[i].y));
+    const float2 den = __ffma2_rn(root.v[i], make_float2(rs, rs), make_float2(a.eps, a.eps));
+    const float2 q = FAST ? __fmul2_rn(m.v[i], make_float2(reciprocal(den.x), reciprocal(den.y)))
+                          : make_float2(m.v[i].x / den.x, m.v[i].y / den.y);
+    const float2 r = __ffma2_rn(make_float2(-ss, -ss), q,
+                                __fmul2_rn(make_float2(p[2 * i], p[2 * i + 1]), make_float2(a.keep, a.keep)));
+    p[2 * i] = r.x;
+    p[2 * i + 1] = r.y;
+  }
+}
+
+// bfloat16 parameters, up or down; ik: first index ^ key
+__device__ __forceinline__ void store_half(bf16* o, bool whole, int n, float (&p)[8], uint32_t ik) {
+  float zero = 0.f;                          // NaN as soon as one of the eight is not finite
+#pragma unroll
+  for (int i = 0; i < 8; ++i) zero = fmaf(p[i], 0.f, zero);
+  if (zero == 0.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = __uint_as_float(__float_as_uint(p[i]) + lower(noise(ik ^ i)));
+  } else {                                   // infinities and NaN keep their bits
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (fabsf(p[i]) < __int_as_float(0x7f800000))
+        p[i] = __uint_as_float(__float_as_uint(p[i]) + lower(noise(ik ^ i)));
+  }
+  if (whole) {                               // the upper halves are the result
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = __byte_perm(__float_as_uint(p[2 * i]), __float_as_uint(p[2 * i + 1]), 0x7632);
+    *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) o[i] = __ushort_as_bfloat16((unsigned short)(__float_as_uint(p[i]) >> 16));
+  }
+}
+
+// 32-bit states: 2048 elements a CTA
+template <int N>
+__global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a) {
+  const int chunk = blockIdx.x, lo = tensor_of(a, chunk);
   const Item& it = a.item[lo];
-  const int64_t c0 = (int64_t)(chunk - (lo > 0 ? a.end[lo - 1] : 0)) * CHUNK;
-  const int lane = threadIdx.x & 31;
-  const bool vec = it.flags & 2, half = it.flags & 1;
-  const int64_t at = c0 + 8 * (int64_t)threadIdx.x;
+  const int64_t at = (int64_t)(chunk - (lo > 0 ? a.end[lo - 1] : 0)) * kChunk + 8 * (int64_t)threadIdx.x;
   const int n = (int)min((int64_t)8, max((int64_t)0, it.n - at));    // elements of this thread
-  // a state's block is whole even where the tensor ends inside it
-  const bool live = at < ((it.n + kBlock - 1) & ~(int64_t)(kBlock - 1));
-  float p[8], g[8];
+  const bool vec = it.flags & 2, half = it.flags & 1;
+  float p[8], g[8], t[8];
   if (half) {
     load_some(static_cast<const bf16*>(it.p) + at, vec, n, p);
     load_some(static_cast<const bf16*>(it.g) + at, vec, n, g);
@@ -193,77 +249,95 @@ __global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a)
     load_some(static_cast<const float*>(it.g) + at, vec, n, g);
   }
   Eight m, v, root;
-  if constexpr (EIGHT) {
-    const float sm = live ? it.ms[at / kBlock] : 0.f, sv = live ? it.vs[at / kBlock] : 0.f;
-    const int64_t in = live ? at : 0;        // lanes past the state read its start and hold nothing
-    m = load_codes(it.m, in, sm);
-    v = load_codes(it.v, in, sv);
+  load_some(static_cast<const float*>(it.m) + at, true, n, t);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m.v[i] = make_float2(t[2 * i], t[2 * i + 1]);
+  load_some(static_cast<const float*>(it.v) + at, true, n, t);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.v[i] = make_float2(t[2 * i], t[2 * i + 1]);
+  update<false>(a, it.step_size, it.root_scale, p, g, m, v, root);
+  if (half)
+    store_half(static_cast<bf16*>(it.p) + at, vec && n >= 8, n, p, (it.first + (uint32_t)at) ^ (it.key + 1));
+  else
+    store_some(static_cast<float*>(it.p) + at, vec, n, p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = m.get(i);
+  store_some(static_cast<float*>(it.m) + at, true, n, t);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = v.get(i);
+  store_some(static_cast<float*>(it.v) + at, true, n, t);
+}
+
+// What a thread of the 8-bit form loads for eight elements, unconverted.
+template <bool HALF>
+struct Ahead {
+  uint4 p[HALF ? 1 : 2], g[HALF ? 1 : 2];
+  uint2 m, v;
+  float sm, sv;
+};
+
+// 8-bit states.  Finding the tensor and its addresses takes a microsecond of
+// dependent reads, a fifth of the time where arithmetic is the bound (184 M bfloat16
+// parameters in 97 tensors 677 us, in one tensor 548): bfloat16 parameters go
+// through kRounds times 2048 elements a CTA, the next ones loaded before the current
+// ones are computed (514 us).  float32 moves 16 bytes a parameter, memory is the
+// bound again, and one round with more CTAs is faster (96 M: 266 us against 299).
+template <int N, bool HALF>
+__device__ __forceinline__ void steps8(const Args<N>& a, const Item& it, int64_t c0) {
+  using T = typename std::conditional<HALF, bf16, float>::type;
+  constexpr int R = HALF ? kRounds : 1;
+  const int lane = threadIdx.x & 31;
+  const int64_t total = it.n, padded = (total + kBlock - 1) & ~(int64_t)(kBlock - 1);
+  const bool vec = it.flags & 2;
+  T* const p0 = static_cast<T*>(it.p);
+  const T* const g0 = static_cast<const T*>(it.g);
+  const uint8_t* const m0 = static_cast<const uint8_t*>(it.m);
+  const uint8_t* const v0 = static_cast<const uint8_t*>(it.v);
+  float *const ms = it.ms, *const vs = it.vs;
+  const uint32_t first = it.first, key = it.key;
+  const float ss = it.step_size, rs = it.root_scale;
+  Ahead<HALF> next;
+  const auto load = [&](int64_t at) {
+    if (vec && at + 8 <= total) {
+#pragma unroll
+      for (int q = 0; q < (HALF ? 1 : 2); ++q) {
+        next.p[q] = *reinterpret_cast<const uint4*>(p0 + at + q * 4);
+        next.g[q] = *reinterpret_cast<const uint4*>(g0 + at + q * 4);
+      }
+    }
+    const bool live = at < padded;           // a state's block is whole even where the tensor ends inside it
+    next.m = live ? *reinterpret_cast<const uint2*>(m0 + at) : make_uint2(0, 0);
+    next.v = live ? *reinterpret_cast<const uint2*>(v0 + at) : make_uint2(0, 0);
+    next.sm = live ? ms[at / kBlock] : 0.f;
+    next.sv = live ? vs[at / kBlock] : 0.f;
+  };
+  int64_t at = c0 + 8 * (int64_t)threadIdx.x;
+  load(at);
+#pragma unroll 1
+  for (int round = 0; round < R; ++round, at += kChunk) {
+    if (c0 + round * (int64_t)kChunk >= total) break;      // the same for the whole CTA
+    const int n = (int)min((int64_t)8, max((int64_t)0, total - at));
+    const bool live = at < padded, whole = vec && n >= 8;
+    float p[8], g[8];
+    if (whole) {
+      load8(reinterpret_cast<const T*>(next.p), p);
+      load8(reinterpret_cast<const T*>(next.g), g);
+    } else {
+      load_some(p0 + at, false, n, p);
+      load_some(g0 + at, false, n, g);
+    }
+    Eight m = decode(next.m, next.sm), v = decode(next.v, next.sv), root;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v.v[i] = __fmul2_rn(v.v[i], v.v[i]);
-  } else {
-    float t[8];
-    load_some(static_cast<const float*>(it.m) + at, true, n, t);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m.v[i] = make_float2(t[2 * i], t[2 * i + 1]);
-    load_some(static_cast<const float*>(it.v) + at, true, n, t);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v.v[i] = make_float2(t[2 * i], t[2 * i + 1]);
-  }
-  const uint32_t i0 = it.first + (uint32_t)at;             // a multiple of 8: i0 + i = i0 ^ i
-  const float2 b1 = make_float2(a.b1, a.b1), c1 = make_float2(a.c1, a.c1);
-  const float2 b2 = make_float2(a.b2, a.b2), c2 = make_float2(a.c2, a.c2);
-  const float ss = it.step_size, rs = it.root_scale;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    // each operation rounded on its own, so that a restatement in elementary
-    // 32-bit operations gives the same states, bit for bit
-    const float2 gg = make_float2(g[2 * i], g[2 * i + 1]);
-    m.v[i] = add_apart(__fmul2_rn(b1, m.v[i]), __fmul2_rn(c1, gg));
-    v.v[i] = add_apart(__fmul2_rn(b2, v.v[i]), __fmul2_rn(__fmul2_rn(c2, gg), gg));
-    root.v[i] = make_float2(sqrtf(v.v[i].x), sqrtf(v.v[i].y));
-    const float2 den = __ffma2_rn(root.v[i], make_float2(rs, rs), make_float2(a.eps, a.eps));
-    // with 8-bit states arithmetic is the bound: the quotient may be two units of
-    // its last place off, far inside a step of either format
-    const float2 q = EIGHT ? __fmul2_rn(m.v[i], make_float2(reciprocal(den.x), reciprocal(den.y)))
-                           : make_float2(m.v[i].x / den.x, m.v[i].y / den.y);
-    const float2 r = __ffma2_rn(make_float2(-ss, -ss), q,
-                                __fmul2_rn(make_float2(p[2 * i], p[2 * i + 1]), make_float2(a.keep, a.keep)));
-    p[2 * i] = r.x;
-    p[2 * i + 1] = r.y;
-  }
-  if (half) {
-    const uint32_t ik = i0 ^ (it.key + 1);
-    float zero = 0.f;                        // NaN as soon as one of the eight is not finite
-#pragma unroll
-    for (int i = 0; i < 8; ++i) zero = fmaf(p[i], 0.f, zero);
-    if (zero == 0.f) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        p[i] = __uint_as_float(__float_as_uint(p[i]) + lower(noise(ik ^ i)));
-    } else {                                 // infinities and NaN keep their bits
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (fabsf(p[i]) < __int_as_float(0x7f800000))
-          p[i] = __uint_as_float(__float_as_uint(p[i]) + lower(noise(ik ^ i)));
-    }
-    bf16* o = static_cast<bf16*>(it.p) + at;
-    if (vec && n >= 8) {                     // the upper halves are the result
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = __byte_perm(__float_as_uint(p[2 * i]), __float_as_uint(p[2 * i + 1]), 0x7632);
-      *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) o[i] = __ushort_as_bfloat16((unsigned short)(__float_as_uint(p[i]) >> 16));
-    }
-  } else {
-    store_some(static_cast<float*>(it.p) + at, vec, n, p);
-  }
-  if constexpr (EIGHT) {
+    if (round + 1 < R) load(at + kChunk);
+    update<true>(a, ss, rs, p, g, m, v, root);
+    const uint32_t i0 = first + (uint32_t)at;              // a multiple of 8: i0 + i = i0 ^ i
+    if constexpr (HALF)
+      store_half(p0 + at, whole, n, p, i0 ^ (key + 1));
+    else
+      store_some(p0 + at, vec, n, p);
     uint32_t h[8];
-    const uint32_t ik = i0 ^ it.key;
+    const uint32_t ik = i0 ^ key;
 #pragma unroll
     for (int i = 0; i < 8; ++i) h[i] = noise(ik ^ i);
     if (n < 8) {                             // past the tensor: held as zero
@@ -273,21 +347,22 @@ __global__ void __launch_bounds__(NT) k_adamw(const __grid_constant__ Args<N> a)
         if (2 * i + 1 >= n) m.v[i].y = root.v[i].y = 0.f;
       }
     }
-    hold<false>(it.m, it.ms, at, live, m, h, lane);
-    hold<true>(it.v, it.vs, at, live, root, h, lane);
-  } else {
-    float t[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = m.get(i);
-    store_some(static_cast<float*>(it.m) + at, true, n, t);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = v.get(i);
-    store_some(static_cast<float*>(it.v) + at, true, n, t);
+    hold<false>(it.m, ms, at, live, m, h, lane);
+    hold<true>(it.v, vs, at, live, root, h, lane);
   }
 }
 
+// one type of parameters a launch: the two forms need 48 and 66 registers
+template <int N, bool HALF>
+__global__ void __launch_bounds__(NT) k_adamw8(const __grid_constant__ Args<N> a) {
+  const int chunk = blockIdx.x, lo = tensor_of(a, chunk);
+  const int64_t c0 = (int64_t)(chunk - (lo > 0 ? a.end[lo - 1] : 0)) * kChunk;
+  steps8<N, HALF>(a, a.item[lo], c0 * (HALF ? kRounds : 1));
+}
+
+// Launches over the tensors `t[i]`, i in `pick`.
 template <int N>
-int launch(const race_adamw_desc_t* d, const race_adamw_tensor_t* t, int count, cudaStream_t s) {
+int launch(const race_adamw_desc_t* d, const race_adamw_tensor_t* t, const int64_t* pick, int count, cudaStream_t s) {
   static_assert(sizeof(Args<N>) <= 32764, "a launch carries 32764 bytes of parameters");
   Args<N> a;
   a.keep = (float)(1.0 - d->lr * d->weight_decay);
@@ -296,14 +371,12 @@ int launch(const race_adamw_desc_t* d, const race_adamw_tensor_t* t, int count, 
   a.b2 = (float)d->beta_two;
   a.c2 = (float)(1.0 - d->beta_two);
   a.eps = (float)d->eps;
+  const bool eight = d->state_bits == 8, half = t[pick[0]].dtype == RACE_BF16;
   int64_t chunks = 0;
-  int used = 0;
   for (int i = 0; i < count; ++i) {
-    const race_adamw_tensor_t& x = t[i];
-    if (x.numel == 0) continue;
+    const race_adamw_tensor_t& x = t[pick[i]];
     const int32_t step = x.step + 1;
-    Item& it = a.item[used];
-    const int es = x.dtype == RACE_BF16 ? 2 : 4;
+    Item& it = a.item[i];
     it.p = x.param;
     it.g = x.grad;
     it.m = x.exp_avg;
@@ -317,21 +390,23 @@ int launch(const race_adamw_desc_t* d, const race_adamw_tensor_t* t, int count, 
     it.root_scale = (float)(1.0 / std::sqrt(1.0 - std::pow(d->beta_two, step)));
     const bool vec = reinterpret_cast<uintptr_t>(x.param) % 16 == 0 &&
                      reinterpret_cast<uintptr_t>(x.grad) % 16 == 0;
-    it.flags = (es == 2 ? 1 : 0) | (vec ? 2 : 0);
-    chunks += (x.numel + CHUNK - 1) / CHUNK;
+    it.flags = (x.dtype == RACE_BF16 ? 1 : 0) | (vec ? 2 : 0);
+    const int64_t each = eight && half ? kChunk * kRounds : kChunk;
+    chunks += (x.numel + each - 1) / each;
     if (chunks >= (int64_t(1) << 31)) {
       api_note("adamw: 2^42 elements and more in one launch");
       return RACE_ERR_UNSUPPORTED;
     }
-    a.end[used++] = (int32_t)chunks;
+    a.end[i] = (int32_t)chunks;
   }
-  a.count = used;
-  if (used == 0) return RACE_OK;
-  if (d->state_bits == 8)
-    k_adamw<N, true><<<(unsigned)chunks, NT, 0, s>>>(a);
+  a.count = count;
+  if (!eight)
+    k_adamw<N><<<(unsigned)chunks, NT, 0, s>>>(a);
+  else if (half)
+    k_adamw8<N, true><<<(unsigned)chunks, NT, 0, s>>>(a);
   else
-    k_adamw<N, false><<<(unsigned)chunks, NT, 0, s>>>(a);
-  api_log(d->state_bits == 8 ? "adamw_8bit" : "adamw");
+    k_adamw8<N, false><<<(unsigned)chunks, NT, 0, s>>>(a);
+  api_log(eight ? "adamw_8bit" : "adamw");
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? RACE_OK : api_cuda_fail(e);
 }
@@ -366,15 +441,20 @@ extern "C" int race_adamw(const race_adamw_desc_t* desc, const race_adamw_tensor
   }
   if (count == 0) return RACE_OK;
   RACE_CALL(api_bind(stream));
-  for (int64_t i = 0; i < count;) {
-    const int64_t left = count - i;
-    if (left <= adamw::kFew) {
-      RACE_CALL(adamw::launch<adamw::kFew>(desc, tensors + i, (int)left, stream));
-      break;
+  // 32-bit states take both types in one launch, 8-bit states one after the other
+  for (int type = 0; type < (desc->state_bits == 8 ? 2 : 1); ++type) {
+    int64_t pick[adamw::kMany];
+    int n = 0;
+    for (int64_t i = 0; i <= count; ++i) {
+      if (i < count && tensors[i].numel > 0 &&
+          (desc->state_bits == 32 || tensors[i].dtype == (type == 0 ? RACE_BF16 : RACE_F32)))
+        pick[n++] = i;
+      if (n == adamw::kMany || (i == count && n > 0)) {
+        RACE_CALL(n <= adamw::kFew ? adamw::launch<adamw::kFew>(desc, tensors, pick, n, stream)
+                                   : adamw::launch<adamw::kMany>(desc, tensors, pick, n, stream));
+        n = 0;
+      }
     }
-    const int now = (int)(left < adamw::kMany ? left : adamw::kMany);
-    RACE_CALL(adamw::launch<adamw::kMany>(desc, tensors + i, now, stream));
-    i += now;
   }
   return RACE_OK;
 }
