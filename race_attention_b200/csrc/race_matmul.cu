@@ -697,38 +697,27 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
       }
       if (*abort != 0) continue;
-      if (p.splits > 1) {
-        // partial results are read once, by the join
-        float* o = p.part + ((int64_t)t.split * a.m + mr) * a.n + n0;
-        if (mr < a.m) {
-          if (n0 + 128 <= a.n && a.n % 4 == 0) {
+      // Two boxes of 32 rows x 128 bytes at a time (bfloat16: all 128 columns), 16-byte
+      // chunk c of row r at c ^ (r % 8).  They leave by TMA, or, where the result's
+      // rows do not start on 16 bytes and for partial results (whose rows a ragged
+      // tile must not leave), row by row with a lane to a column.
+      const int r0 = (int)(mr - lane);
+      const bool tma = p.splits == 1 && p.store;
+      if (p.splits == 1 && a.ybf16) {
+        if (lane == 0) store_wait_read();                          // the last tile's stores have read the boxes
+        __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 128; j += 4)
-              *reinterpret_cast<float4*>(o + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-          } else {
+        for (int c = 0; c < 16; ++c) {
+          uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < 128; ++j)
-              if (n0 + j < a.n) o[j] = acc[j];
+          for (int q = 0; q < 4; ++q) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(acc[8 * c + 2 * q], acc[8 * c + 2 * q + 1]);
+            w[q] = *reinterpret_cast<const uint32_t*>(&h);
           }
+          *reinterpret_cast<uint4*>(box + (c >> 3) * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
         }
-      } else if (p.store) {
-        // Two boxes of 32 rows x 128 bytes at a time (bfloat16: all 128 columns),
-        // 16-byte chunk c of row r at c ^ (r % 8).
-        const int r0 = (int)(mr - lane);
-        if (a.ybf16) {
-          if (lane == 0) store_wait_read();                        // the last tile's stores have read the boxes
-          __syncwarp();
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            uint32_t w[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const __nv_bfloat162 h = __floats2bfloat162_rn(acc[8 * c + 2 * q], acc[8 * c + 2 * q + 1]);
-              w[q] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            *reinterpret_cast<uint4*>(box + (c >> 3) * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
-          }
+        if (tma) {
           t5::fence_async_smem();
           __syncwarp();
           if (lane == 0 && r0 < a.m) {
@@ -737,29 +726,52 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         } else {
+          __syncwarp();
+          bf16* o = static_cast<bf16*>(a.y) + r0 * a.ldy + n0;
+          const int rows = (int)min((int64_t)32, a.m - r0), cols = (int)min((int64_t)128, a.n - n0);
+          for (int r = 0; r < rows; ++r, o += a.ldy)
 #pragma unroll
-          for (int g = 0; g < 4; g += 2) {
-            if (lane == 0) store_wait_read();
-            __syncwarp();
+            for (int h = 0; h < 4; ++h) {
+              const int c = lane + 32 * h;
+              if (c < cols)
+                o[c] = *reinterpret_cast<const bf16*>(box + (h >> 1) * 4096 + r * 128 +
+                                                      ((((c >> 3) & 7) ^ (r & 7)) << 4) + (c & 7) * 2);
+            }
+          __syncwarp();
+        }
+      } else {
 #pragma unroll
-            for (int c = 0; c < 16; ++c)
-              *reinterpret_cast<float4*>(box + (c >> 3) * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) =
-                  make_float4(acc[32 * g + 4 * c], acc[32 * g + 4 * c + 1], acc[32 * g + 4 * c + 2],
-                              acc[32 * g + 4 * c + 3]);
+        for (int g = 0; g < 4; g += 2) {
+          if (lane == 0) store_wait_read();
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 16; ++c)
+            *reinterpret_cast<float4*>(box + (c >> 3) * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) =
+                make_float4(acc[32 * g + 4 * c], acc[32 * g + 4 * c + 1], acc[32 * g + 4 * c + 2],
+                            acc[32 * g + 4 * c + 3]);
+          const int64_t col = n0 + 32 * g;
+          if (tma) {
             t5::fence_async_smem();
             __syncwarp();
-            const int64_t col = n0 + 32 * g;
             if (lane == 0 && r0 < a.m) {
               if (col < a.n) tma2_store(&mapy, (int)col * 4, r0, saddr(box));
               if (col + 32 < a.n) tma2_store(&mapy, (int)col * 4 + 128, r0, saddr(box) + 4096);
             }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          } else {
+            __syncwarp();
+            const int64_t ld = p.splits > 1 ? a.n : a.ldy;
+            float* o = (p.splits > 1 ? p.part + (int64_t)t.split * a.m * a.n : static_cast<float*>(a.y)) + r0 * ld + col;
+            const int rows = (int)min((int64_t)32, a.m - r0), cols = (int)min((int64_t)64, a.n - col);
+            for (int r = 0; r < rows; ++r, o += ld)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (lane + 32 * h < cols)
+                  o[lane + 32 * h] = *reinterpret_cast<const float*>(box + h * 4096 + r * 128 +
+                                                                     (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+            __syncwarp();
           }
         }
-      } else if (mr < a.m) {
-#pragma unroll
-        for (int j = 0; j < 128; ++j)
-          if (n0 + j < a.n) put(a, mr, n0 + j, acc[j]);
       }
     }
     if (lane == 0) store_wait_read();

@@ -129,6 +129,11 @@ Tensor matmul(const Tensor& ac, const Tensor& as, const Tensor& bc, const Tensor
                  out.has_value() ? *out : Tensor());
 }
 
+// The gradients are computed outside torch, so they have none of their own.
+void once() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "the 8-bit operators have no second derivatives (create_graph=True)");
+}
+
 struct Linear : torch::autograd::Function<Linear> {
   // x [..., K]; weight [N, K], or none with its held form (codes, scales and those of its transpose)
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& weight, const Maybe& wc, const Maybe& ws,
@@ -154,6 +159,7 @@ struct Linear : torch::autograd::Function<Linear> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once();
     const variable_list saved = ctx->get_saved_variables();
     auto* status = reinterpret_cast<uint32_t*>(ctx->saved_data["status"].toInt());
     const bool need_x = ctx->saved_data["need_x"].toBool() && ctx->needs_input_grad(0);
@@ -215,6 +221,7 @@ struct Norm : torch::autograd::Function<Norm> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once();
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &h = saved[0], &w = saved[1], &rstd = saved[2];
     const Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();

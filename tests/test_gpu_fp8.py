@@ -495,6 +495,14 @@ def test_norm_layouts_types_and_edges():
     assert torch.equal(*grads)
 
 
+def test_no_second_derivatives():
+    from race_attention_b200.fp8 import fp8_linear, rms_norm
+    x, w = torch.ones(4, 64, device="cuda", requires_grad=True), torch.ones(32, 64, device="cuda", requires_grad=True)
+    for y in (fp8_linear(x, w), rms_norm(x, w[0])):
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 def test_norm_refusals():
     from race_attention_b200.fp8 import rms_norm
     x, w = torch.ones(2, 64, device="cuda"), torch.ones(64, device="cuda")
