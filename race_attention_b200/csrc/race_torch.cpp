@@ -121,11 +121,22 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> quantize(const Tensor& x, bool square
   return {a.codes, a.scales, t.codes, t.scales};
 }
 
-Tensor matmul(const Tensor& ac, const Tensor& as, const Tensor& bc, const Tensor& bs, bool square, bool f32,
-              const Maybe& out, int64_t status) {
+Tensor matmul(const Tensor& ac, const Tensor& as, bool a_square, const Tensor& bc, const Tensor& bs, bool b_square,
+              bool f32, const Maybe& out, int64_t status) {
+  TORCH_CHECK_VALUE(!a_square, "a must have a scale for each row; only b may have square blocks");
+  TORCH_CHECK_VALUE(ac.size(1) == bc.size(1), "a ", ac.sizes(), " and b ", bc.sizes(),
+                    " must have the same number of columns");
+  TORCH_CHECK_VALUE(ac.device() == bc.device(), "a and b must be on the same device");
+  if (out.has_value()) {
+    const int64_t m = ac.size(0), n = bc.size(0);
+    TORCH_CHECK_VALUE(out->dim() == 2 && out->size(0) == m && out->size(1) == n && out->device() == ac.device() &&
+                          out->scalar_type() == (f32 ? at::kFloat : at::kBFloat16) &&
+                          (n <= 1 || out->stride(1) == 1) && (m <= 1 || out->stride(0) >= n),
+                      "out must be a [", m, ", ", n, "] tensor of out_dtype with contiguous columns");
+  }
   c10::cuda::CUDAGuard guard(ac.device());
   at::NoGradGuard no_grad;
-  return product(in_place({ac, as}), in_place({bc, bs}), square, f32, reinterpret_cast<uint32_t*>(status),
+  return product(in_place({ac, as}), in_place({bc, bs}), b_square, f32, reinterpret_cast<uint32_t*>(status),
                  out.has_value() ? *out : Tensor());
 }
 

@@ -57,17 +57,14 @@ class BlockFp8:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype != F8 or codes.dim() != 2:
             raise ValueError("codes must be a 2-D torch.float8_e4m3fn tensor")
+        if scales.dtype != torch.float32 or scales.device != codes.device or scales.dim() != 2:
+            raise ValueError("scales must be a 2-D float32 tensor on the codes' device")
         r, k = codes.shape
-        if scales.dtype != torch.float32 or scales.device != codes.device:
-            raise ValueError("scales must be float32 on the codes' device")
-        shape = tuple(scales.shape)
-        if shape == (r, _blocks_of(k)):
-            self.square = False
-        elif shape == (_blocks_of(r), _blocks_of(k)):
-            self.square = True
-        else:
+        sr, sk = scales.shape
+        if sk != -(-k // BLOCK) or (sr != r and sr != -(-r // BLOCK)):
             raise ValueError(f"scales of codes [{r}, {k}] must be [{r}, {_blocks_of(k)}] or "
-                             f"[{_blocks_of(r)}, {_blocks_of(k)}], got {list(shape)}")
+                             f"[{_blocks_of(r)}, {_blocks_of(k)}], got {list(scales.shape)}")
+        self.square = sr != r
         self.codes, self.scales = codes, scales
 
     @property
@@ -118,24 +115,13 @@ def fp8_matmul(a: BlockFp8, b: BlockFp8, out_dtype: torch.dtype = torch.bfloat16
     128 x 128 block.  Each 128-long partial product is scaled and summed in 32
     bits, in an order that depends on the shape alone.  out: a [M, N] tensor to
     write (any row stride, contiguous columns), of the result's type."""
-    ac, bc = a.codes, b.codes
-    if a.square:
-        raise ValueError("a must have a scale for each row; only b may have square blocks")
-    if ac.shape[1] != bc.shape[1]:
-        raise ValueError(f"a {list(ac.shape)} and b {list(bc.shape)} must have the same number of columns")
-    if bc.device != ac.device:
-        raise ValueError("a and b must be on the same device")
     if out_dtype not in _SUPPORTED:
         raise ValueError("out_dtype must be float32 or bfloat16")
-    if not ac.is_cuda:
+    codes = a.codes
+    if not codes.is_cuda:
         raise RuntimeError("fp8_matmul runs on CUDA devices only (no CPU fallback)")
-    if out is not None:
-        m, n = ac.shape[0], bc.shape[0]
-        if (out.shape != (m, n) or out.dtype != out_dtype or out.device != ac.device
-                or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n)):
-            raise ValueError(f"out must be a [{m}, {n}] {out_dtype} tensor with contiguous columns")
-    return _ops.matmul(ac, a.scales, bc, b.scales, b.square, out_dtype == torch.float32, out,
-                       host_status.word(ac.device))
+    return _ops.matmul(codes, a.scales, a.square, b.codes, b.scales, b.square, out_dtype == torch.float32,
+                       out, host_status.word(codes.device))
 
 
 Weight = Union[torch.Tensor, BlockFp8, Tuple[BlockFp8, BlockFp8]]

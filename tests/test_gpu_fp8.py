@@ -233,6 +233,30 @@ def test_product_on_another_stream_and_in_a_graph():
     assert torch.equal(out, ref)
 
 
+@pytest.mark.parametrize("rows", [1, 20, 100])
+def test_products_in_a_row(rows):
+    """Launches that prepare while the one before them ends still see its results:
+    each product's input is the last one's, and the run is the same with a
+    synchronisation after each call."""
+    from race_attention_b200.fp8 import fp8_matmul, quantize_fp8
+    w = [quantize_fp8((randn(512, 512, seed=s) / 512 ** 0.5).cuda(), square=True) for s in range(3)]
+
+    def run(sync):
+        x = quantize_fp8(randn(rows, 512, seed=9).cuda())
+        outs = []
+        for i in range(60):
+            y = fp8_matmul(x, w[i % 3])
+            # a product of the same inputs right behind it, into memory that is reused
+            fp8_matmul(x, w[(i + 1) % 3])
+            x = quantize_fp8(y)
+            outs.append(y)
+            if sync:
+                torch.cuda.synchronize()
+        return torch.stack(outs)
+
+    assert torch.equal(run(False), run(True))
+
+
 @pytest.mark.parametrize("m", [8, 1000])
 def test_product_wait_limit(m):
     """A wait that runs out is reported, and the next call is whole again."""
