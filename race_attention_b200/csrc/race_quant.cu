@@ -6,9 +6,10 @@
 // pass, which memory bounds (bf16: 2 bytes read and 2 written per element).
 // A CTA takes a 128 x 128 tile, a whole block in either direction; thread
 // (ty, tx) holds rows 8 ty .. 8 ty + 7 of columns 8 tx .. 8 tx + 7 in registers, so the tile
-// never passes through shared memory at full width: a row's maximum is taken
-// over the 16 lanes of a half warp, a column's over the thread's rows and then
-// eight warps.  Transposed codes are packed eight rows to a word pair in
+// never passes through shared memory at full width: the maxima of the eight rows
+// are taken over the 16 lanes of a half warp in one exchange that leaves each
+// pair of lanes with one row (and one reciprocal to form), a column's over the
+// thread's rows and then eight warps.  Transposed codes are packed eight rows to a word pair in
 // registers and cross shared memory as bytes (16 KB), written out in whole
 // 128-byte rows.
 #include "race_api.h"
@@ -39,19 +40,21 @@ struct Tile<float> {
   __device__ __forceinline__ void load(int i, const float* p) { load8(p, v[i]); }
   __device__ __forceinline__ void set(int i, int j, float x) { v[i][j] = x; }
   __device__ __forceinline__ float get(int i, int j) const { return v[i][j]; }
+  // magnitudes are compared as they are; a column word holds one of them
+  static constexpr int CW = 8;
+  static __device__ __forceinline__ uint32_t bits(uint32_t m) { return m; }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
   __device__ __forceinline__ uint32_t row_max(int i) const {
     uint32_t m = mag(v[i][0]);
 #pragma unroll
     for (int j = 1; j < 8; ++j) m = max(m, mag(v[i][j]));
     return m;
   }
-  __device__ __forceinline__ void col_max(uint32_t (&m)[8]) const {
+  __device__ __forceinline__ uint32_t col_max(int j) const {
+    uint32_t m = mag(v[0][j]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      m[j] = mag(v[0][j]);
-#pragma unroll
-      for (int i = 1; i < 8; ++i) m[j] = max(m[j], mag(v[i][j]));
-    }
+    for (int i = 1; i < 8; ++i) m = max(m, mag(v[i][j]));
+    return m;
   }
 };
 
@@ -69,27 +72,36 @@ struct Tile<bf16> {
   __device__ __forceinline__ float get(int i, int j) const {
     return __uint_as_float((j & 1) ? w[i][j >> 1] & 0xffff0000u : w[i][j >> 1] << 16);
   }
-  // the larger magnitudes of two pairs, NaN if there is one
-  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hmax2_nan(__habs2(reinterpret_cast<const __nv_bfloat162&>(a)),
-                                         __habs2(reinterpret_cast<const __nv_bfloat162&>(b)));
-    return reinterpret_cast<const uint32_t&>(r);
-  }
+  // magnitudes are compared as 16-bit integers, two to a word
+  static constexpr int CW = 4;
+  static __device__ __forceinline__ uint32_t bits(uint32_t m) { return m << 16; }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+  __device__ __forceinline__ uint32_t two(int i, int q) const { return w[i][q] & 0x7fff7fffu; }
   __device__ __forceinline__ uint32_t row_max(int i) const {
-    const uint32_t m = max2(max2(w[i][0], w[i][1]), max2(w[i][2], w[i][3]));
-    return max(m & 0x7fff0000u, m << 16 & 0x7fff0000u);
+    const uint32_t m = larger(larger(two(i, 0), two(i, 1)), larger(two(i, 2), two(i, 3)));
+    return max(m & 0xffffu, m >> 16);
   }
-  __device__ __forceinline__ void col_max(uint32_t (&m)[8]) const {
+  __device__ __forceinline__ uint32_t col_max(int q) const {
+    uint32_t m = two(0, q);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint32_t t = w[0][q];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) t = max2(t, w[i][q]);
-      m[2 * q] = t << 16 & 0x7fff0000u;
-      m[2 * q + 1] = t & 0x7fff0000u;
-    }
+    for (int i = 1; i < 8; ++i) m = larger(m, two(i, q));
+    return m;
   }
 };
+
+// The maxima over a half warp of eight values a lane: every step hands half of the
+// values over, so that eight exchanges do, and lane tx ends with that of row tx / 2.
+__device__ __forceinline__ uint32_t max_of_row(const uint32_t (&m)[8], int tx) {
+  uint32_t a[4], b[2], c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    a[i] = max(tx & 8 ? m[4 + i] : m[i], __shfl_xor_sync(0xffffffffu, tx & 8 ? m[i] : m[4 + i], 8));
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    b[i] = max(tx & 4 ? a[2 + i] : a[i], __shfl_xor_sync(0xffffffffu, tx & 4 ? a[i] : a[2 + i], 4));
+  c = max(tx & 2 ? b[1] : b[0], __shfl_xor_sync(0xffffffffu, tx & 2 ? b[0] : b[1], 2));
+  return max(c, __shfl_xor_sync(0xffffffffu, c, 1));
+}
 
 template <typename T>
 __device__ __forceinline__ uint2 code_row(const Tile<T>& t, int i, float inv) {
@@ -102,7 +114,8 @@ __device__ __forceinline__ uint2 code_row(const Tile<T>& t, int i, float inv) {
 template <typename T, bool VEC, bool SQUARE, bool ROWS, bool COLS>
 __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_quantize(const Args a) {
   __shared__ __align__(16) uint2 tile[COLS ? 128 * 16 : 1];   // [column][8-row group], swizzled
-  __shared__ uint32_t wmax[8][COLS && !SQUARE ? 128 : 1];
+  constexpr int CW = Tile<T>::CW;                              // words of 8 columns' maxima
+  __shared__ uint32_t wmax[8][COLS && !SQUARE ? 16 * CW : 1];
   __shared__ float cinv[COLS && !SQUARE ? 128 : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tx = tid & 15, ty = tid >> 4;
@@ -127,21 +140,27 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_quantize(const A
     }
   }
   if constexpr (COLS && !SQUARE) {
-    uint32_t m[8];
-    v.col_max(m);
+    uint32_t m[CW];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+    for (int q = 0; q < CW; ++q) {
+      m[q] = v.col_max(q);
+      m[q] = Tile<T>::larger(m[q], __shfl_xor_sync(0xffffffffu, m[q], 16));
+    }
     if (lane < 16)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) wmax[warp][8 * tx + j] = m[j];
+      for (int q = 0; q < CW; ++q) wmax[warp][CW * tx + q] = m[q];
     __syncthreads();
-    if (tid < 128) {
+    if (tid < 16 * CW) {
       uint32_t t = wmax[0][tid];
 #pragma unroll
-      for (int w = 1; w < 8; ++w) t = max(t, wmax[w][tid]);
-      const float s = scale_of(t);
-      cinv[tid] = 1.f / s;
-      if (c0 + tid < a.cols) a.cs[(c0 + tid) * a.csr + blockIdx.y * a.csb] = s;
+      for (int w = 1; w < 8; ++w) t = Tile<T>::larger(t, wmax[w][tid]);
+#pragma unroll
+      for (int z = 0; z < 8 / CW; ++z) {                       // bfloat16: two columns a word
+        const int col = tid * (8 / CW) + z;
+        const float s = scale_of(Tile<T>::bits(CW == 8 ? t : z ? t >> 16 : t & 0xffffu));
+        cinv[col] = 1.f / s;
+        if (c0 + col < a.cols) a.cs[(c0 + col) * a.csr + blockIdx.y * a.csb] = s;
+      }
     }
   }
   uint2 code[SQUARE ? 8 : 1];
@@ -154,7 +173,7 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_quantize(const A
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; ++w) m = max(m, wmax[w][0]);
-    const float s = scale_of(m), inv = 1.f / s;
+    const float s = scale_of(Tile<T>::bits(m)), inv = 1.f / s;
     if (tid == 0) {
       if (ROWS) a.rs[blockIdx.y * a.rsr + blockIdx.x * a.rsb] = s;
       if (COLS && a.cs != nullptr) a.cs[blockIdx.x * a.csr + blockIdx.y * a.csb] = s;
@@ -165,15 +184,22 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_quantize(const A
   if constexpr (ROWS) {
     // the pitch is a multiple of 16: whole 8-byte groups fit
     const bool in = c < ((a.cols + 15) & ~int64_t(15));
+    float rinv = 0.f;
+    if constexpr (!SQUARE) {
+      uint32_t m[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m[i] = v.row_max(i);
+      const float s = scale_of(Tile<T>::bits(max_of_row(m, tx)));
+      rinv = 1.f / s;
+      if ((tx & 1) == 0 && r + (tx >> 1) < a.rows) a.rs[(r + (tx >> 1)) * a.rsr + blockIdx.x * a.rsb] = s;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint2 q;
       if constexpr (SQUARE) {
         q = code[i];
       } else {
-        const float s = scale_of(max_over(v.row_max(i), 16));
-        if (tx == 0 && r + i < a.rows) a.rs[(r + i) * a.rsr + blockIdx.x * a.rsb] = s;
-        q = code_row(v, i, 1.f / s);
+        q = code_row(v, i, __shfl_sync(0xffffffffu, rinv, 2 * i, 16));
       }
       if (r + i < a.rows && in) *reinterpret_cast<uint2*>(a.rc + (r + i) * a.ldr + c) = q;
     }
