@@ -443,8 +443,8 @@ struct Pair {
   static constexpr int A = 128 * 128, STAGE = 2 * A;               // this CTA's rows of a and of b
   static constexpr int S = SQ ? 5 : 4;
   static constexpr int OUT = S * STAGE;                            // [8 warps][2] boxes of 32 x 128 bytes
-  static constexpr int SCALES = OUT + 16 * 4096;                   // [2][256] floats (rows of b)
-  static constexpr int BARS = SCALES + (SQ ? 0 : 2048);            // full, empty [S]; tfull, tempty [2]; drain
+  static constexpr int SCALES = OUT + 16 * 4096;                   // rows of b: [8 warps][2][128] floats
+  static constexpr int BARS = SCALES + (SQ ? 0 : 8192);            // full, empty [S]; tfull, tempty [2]; drain
   static constexpr int MISC = BARS + (2 * S + 5) * 8;              // tmem base, abort word, loads issued
   static constexpr int BYTES = MISC + 16 + 1024;
   static_assert(BYTES <= 232448, "227 KB of shared memory");
@@ -635,20 +635,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t lanes = tm + ((uint32_t)(32 * quarter) << 16) + 128 * part;
     const uint32_t te = map_rank(saddr(tempty), 0), tf = saddr(tfull);
     uint8_t* box = sm + L::OUT + (warp - 4) * 8192;
-    float* sbs = reinterpret_cast<float*>(sm + L::SCALES) + 128 * part;
+    float* sbs = reinterpret_cast<float*>(sm + L::SCALES) + 256 * (warp - 4);
     int it = 0;
     // A tile's scales: this thread's row of a, and of b the 128 columns' block
-    // (square) or column `row`.  The next tile and its first scales are found during
-    // this one's first block: in the epilogue they would stand in the way.
-    const float *sa = nullptr, *sb = nullptr, *nsa = nullptr, *nsb = nullptr;
-    float na = 0.f, nb = 0.f, fa = 0.f, fb = 0.f;
+    // (square) or columns lane, 32 + lane, ...: each warp keeps its own copy of the
+    // 128, so that no barrier stands between blocks.  The next tile and its first
+    // scales are found during this one's first block: in the epilogue they would
+    // stand in the way.
+    constexpr int NB = SQ ? 1 : 4;
+    const float *sa = nullptr, *nsa = nullptr, *sb[NB] = {}, *nsb[NB] = {};
+    float na = 0.f, fa = 0.f, nb[NB] = {}, fb[NB] = {};
     Item next = item_of(p, cluster);
     const auto fetch = [&]() {
       const int64_t mr = (int64_t)next.m * 256 + rank * 128 + row, n0 = (int64_t)next.n * 256 + 128 * part;
       nsa = a.sa + (mr < a.m ? mr : a.m - 1) * a.sar + next.k0 * a.sab;
-      nsb = a.sb + (SQ ? min(n0, a.n - 1) / 128 : min(n0 + row, a.n - 1)) * a.sbr + next.k0 * a.sbb;
       fa = __ldg(nsa);
-      fb = __ldg(nsb);
+#pragma unroll
+      for (int q = 0; q < NB; ++q) {
+        nsb[q] = a.sb + (SQ ? min(n0, a.n - 1) / 128 : min(n0 + 32 * q + lane, a.n - 1)) * a.sbr + next.k0 * a.sbb;
+        fb[q] = __ldg(nsb[q]);
+      }
     };
     if (cluster < items) fetch();
     for (int i = cluster; i < items; i += clusters) {
@@ -656,29 +662,43 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int64_t mr = (int64_t)t.m * 256 + rank * 128 + row;    // this thread's row of the result
       const int64_t n0 = (int64_t)t.n * 256 + 128 * part;          // its first column
       sa = nsa;
-      sb = nsb;
       na = fa;
-      nb = fb;
+#pragma unroll
+      for (int q = 0; q < NB; ++q) {
+        sb[q] = nsb[q];
+        nb[q] = fb[q];
+      }
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
       for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
         const int b = it & 1;
-        const float ca = na, cb = nb;
-        const float* sbb = sbs + 256 * b;
+        const float ca = na, cb = nb[0];
+        float* sbb = sbs + 128 * b;
         if constexpr (!SQ) {
-          sbs[256 * b + row] = cb;
-          asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");   // the four warps of these columns
+#pragma unroll
+          for (int q = 0; q < NB; ++q) sbb[32 * q + lane] = nb[q];
+          __syncwarp();
         }
         if (kb + 1 < t.k1) {
           sa += a.sab;
-          sb += a.sbb;
           na = __ldg(sa);
-          nb = __ldg(sb);
+#pragma unroll
+          for (int q = 0; q < NB; ++q) {
+            sb[q] += a.sbb;
+            nb[q] = __ldg(sb[q]);
+          }
         }
         if (kb == t.k0 && i + clusters < items) {
           next = item_of(p, i + clusters);
           fetch();
+        }
+        // rows of b: 16 columns' scales at a time, read while the columns before them
+        // are added (their latency would otherwise stand before each addition)
+        float4 w[2][4];
+        if constexpr (!SQ) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) w[0][q] = *reinterpret_cast<const float4*>(sbb + 4 * q);
         }
         // a wait that ran out leaves garbage here, which is not stored
         wait(tf + 8 * b, (it >> 1) & 1, abort, a.polls);
@@ -694,6 +714,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           t5::tld_wait();
           if (c < 112) {
             t5::tld16(lanes + b * 256 + c + 16, v[cur ^ 1]);
+            if constexpr (!SQ) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) w[cur ^ 1][q] = *reinterpret_cast<const float4*>(sbb + c + 16 + 4 * q);
+            }
           } else {
             fence_before();
             __syncwarp();
@@ -703,8 +727,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           for (int q = 0; q < 16; q += 2) {
             float2 s2 = make_float2(sc, sc);
             if constexpr (!SQ) {
-              const float2 w = *reinterpret_cast<const float2*>(sbb + c + q);
-              s2 = __fmul2_rn(make_float2(ca, ca), w);
+              const float4 f = w[cur][q >> 2];
+              s2 = __fmul2_rn(make_float2(ca, ca), q & 2 ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
             }
             const float2 r = __ffma2_rn(s2, make_float2(v[cur][q], v[cur][q + 1]),
                                         make_float2(acc[c + q], acc[c + q + 1]));
