@@ -57,6 +57,7 @@ struct Args {
   void* y; int64_t ldy; int ybf16;
   int64_t m, n;
   int kb;                                // 128-long blocks of the contraction
+  int ranks;                             // k_mm_split: CTAs of a cluster
   int polls;
   unsigned* status;
 };
@@ -204,8 +205,8 @@ __global__ void __launch_bounds__(kSplitThreads)
   uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::MISC);
   volatile uint32_t* abort = misc + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int C = (int)gridDim.x, rank = (int)blockIdx.x;            // the cluster spans x
-  const int64_t n0 = (int64_t)blockIdx.y * 128, m0 = (int64_t)blockIdx.z * NT;
+  const int C = a.ranks, tile = (int)blockIdx.x / C, rank = (int)blockIdx.x - tile * C;
+  const int64_t n0 = (int64_t)blockIdx.y * 128, m0 = (int64_t)tile * NT;
   const int k0 = (int)((int64_t)a.kb * rank / C), k1 = (int)((int64_t)a.kb * (rank + 1) / C);
   const int blocks = k1 - k0;
 
@@ -398,14 +399,14 @@ int allow_smem(const void* fn, int bytes, std::atomic<uint64_t>& ready) {
 }
 
 template <int NT>
-int launch_split(const Args& a, const CUtensorMap& mw, const CUtensorMap& mx, bool square, int c,
+int launch_split(const Args& a, const CUtensorMap& mw, const CUtensorMap& mx, bool square,
                  cudaStream_t s) {
   void (*fn)(CUtensorMap, CUtensorMap, Args) =
       square ? k_mm_split<NT, true> : k_mm_split<NT, false>;
   static std::atomic<uint64_t> ready[2];
   RACE_CALL(allow_smem(reinterpret_cast<const void*>(fn), Split<NT>::BYTES, ready[square]));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)c, (unsigned)((a.n + 127) / 128), (unsigned)((a.m + NT - 1) / NT));
+  cfg.gridDim = dim3((unsigned)(a.ranks * ((a.m + NT - 1) / NT)), (unsigned)((a.n + 127) / 128));
   cfg.blockDim = dim3(kSplitThreads);
   cfg.dynamicSmemBytes = Split<NT>::BYTES;
   cfg.stream = s;
@@ -413,7 +414,7 @@ int launch_split(const Args& a, const CUtensorMap& mw, const CUtensorMap& mx, bo
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)c;
+  at[0].val.clusterDim.x = (unsigned)a.ranks;
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
@@ -998,8 +999,9 @@ extern "C" int race_scaled_matmul(const race_matmul_desc_t* desc, race_blocks_t 
   RACE_CALL(mm::check_operand(b, desc->n, desc->k));
   mm::Args g{a.scales, a.stride_row, a.stride_block, b.scales, b.stride_row, b.stride_block,
              result.data, result.ld, desc->out_dtype == RACE_BF16, desc->m, desc->n,
-             (int)((desc->k + 127) / 128), desc->wait_polls > 0 ? desc->wait_polls : mm::kPolls, status};
+             (int)((desc->k + 127) / 128), 1, desc->wait_polls > 0 ? desc->wait_polls : mm::kPolls, status};
   const mm::Plan plan = mm::plan_of(desc->m, desc->n, desc->k);
+  g.ranks = plan.c;
   const bool square = desc->b_square != 0;
   CUtensorMap ma, mb;
   if (plan.pair) {
@@ -1022,17 +1024,12 @@ extern "C" int race_scaled_matmul(const race_matmul_desc_t* desc, race_blocks_t 
     return square ? mm::launch_pair<true>(p, ma, mb, my, stream)
                   : mm::launch_pair<false>(p, ma, mb, my, stream);
   }
-  const int64_t tm = (desc->m + plan.nt - 1) / plan.nt, tn = (desc->n + 127) / 128;
-  if (tm > 65535 || tn > 65535) {
-    api_note("matmul: more than 65535 tiles along one side");
-    return RACE_ERR_UNSUPPORTED;
-  }
   if (!api_encode_bytes(&mb, b.codes, desc->n, desc->k, b.ld, 128) ||
       !api_encode_bytes(&ma, a.codes, desc->m, desc->k, a.ld, plan.nt))
     return RACE_ERR_UNSUPPORTED;
   switch (plan.nt) {
-    case 16: return mm::launch_split<16>(g, mb, ma, square, plan.c, stream);
-    case 32: return mm::launch_split<32>(g, mb, ma, square, plan.c, stream);
-    default: return mm::launch_split<64>(g, mb, ma, square, plan.c, stream);
+    case 16: return mm::launch_split<16>(g, mb, ma, square, stream);
+    case 32: return mm::launch_split<32>(g, mb, ma, square, stream);
+    default: return mm::launch_split<64>(g, mb, ma, square, stream);
   }
 }

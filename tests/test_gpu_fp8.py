@@ -172,6 +172,20 @@ def test_product_large(m, n, k, square):
     assert isinstance(B, BlockFp8)
 
 
+def test_product_of_millions_of_rows():
+    """More row tiles than a grid has along its second axis, with few columns."""
+    from race_attention_b200.fp8 import fp8_matmul, quantize_fp8
+    m = 65536 * 64 + 5
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(m, 32, generator=g, device="cuda").bfloat16()
+    w = torch.randn(8, 32, generator=g, device="cuda")
+    A, B = quantize_fp8(x), quantize_fp8(w, square=True)
+    y = fp8_matmul(A, B, torch.float32)
+    ref = A.dequantize() @ B.dequantize().t()
+    assert float((y - ref).norm() / ref.norm()) < L2 + 32 * 2.0 ** -24     # the reference sums in 32 bits too
+    assert float((y[-70:] - ref[-70:]).norm() / ref[-70:].norm()) < L2 + 32 * 2.0 ** -24
+
+
 def test_product_layouts():
     """Scales of either order, codes off 16 bytes or with strided columns, a strided result."""
     from race_attention_b200.fp8 import BlockFp8, fp8_matmul
