@@ -159,12 +159,11 @@ struct Linear : torch::autograd::Function<Linear> {
     if (need_x || need_w) {
       ctx->save_for_backward({need_w ? xt.codes : Tensor(), need_w ? xt.scales : Tensor(),
                               need_x ? t.codes : Tensor(), need_x ? t.scales : Tensor()});
-      ctx->saved_data["status"] = status;
-      ctx->saved_data["x_f32"] = x.scalar_type() == at::kFloat;
-      ctx->saved_data["w_f32"] = weight.has_value() && weight->scalar_type() == at::kFloat;
-      ctx->saved_data["shape"] = x.sizes().vec();
-      ctx->saved_data["need_x"] = need_x;
-      ctx->saved_data["need_w"] = need_w;
+      // status word, types and needs, then x's sizes
+      std::vector<int64_t> meta{status, x.scalar_type() == at::kFloat,
+                                weight.has_value() && weight->scalar_type() == at::kFloat, need_x, need_w};
+      meta.insert(meta.end(), x.sizes().begin(), x.sizes().end());
+      ctx->saved_data["meta"] = meta;
     }
     return y.view(shape);
   }
@@ -172,18 +171,18 @@ struct Linear : torch::autograd::Function<Linear> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once();
     const variable_list saved = ctx->get_saved_variables();
-    auto* status = reinterpret_cast<uint32_t*>(ctx->saved_data["status"].toInt());
-    const bool need_x = ctx->saved_data["need_x"].toBool() && ctx->needs_input_grad(0);
-    const bool need_w = ctx->saved_data["need_w"].toBool() && ctx->needs_input_grad(1);
+    const std::vector<int64_t> meta = ctx->saved_data["meta"].toIntVector();
+    auto* status = reinterpret_cast<uint32_t*>(meta[0]);
+    const bool need_x = meta[3] && ctx->needs_input_grad(0), need_w = meta[4] && ctx->needs_input_grad(1);
     Tensor dx, dw;
     if (grads[0].defined() && (need_x || need_w)) {
       c10::cuda::CUDAGuard guard(grads[0].device());
       const auto [r, c] = quantize_rows(rows_of(grads[0]), false, need_x ? need_w ? kBoth : kRows : kCols);
       if (need_x)
-        dx = product(r, in_place({saved[2], saved[3]}), true, ctx->saved_data["x_f32"].toBool(), status, Tensor())
-                 .view(ctx->saved_data["shape"].toIntVector());
+        dx = product(r, in_place({saved[2], saved[3]}), true, meta[1] != 0, status, Tensor())
+                 .view(at::IntArrayRef(meta).slice(5));
       if (need_w)
-        dw = product(c, {saved[0], saved[1]}, false, ctx->saved_data["w_f32"].toBool(), status, Tensor());
+        dw = product(c, {saved[0], saved[1]}, false, meta[2] != 0, status, Tensor());
     }
     return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -192,9 +191,16 @@ struct Linear : torch::autograd::Function<Linear> {
 Tensor linear(const Tensor& x, const Maybe& weight, const Maybe& wc, const Maybe& ws, const Maybe& tc, const Maybe& ts,
               bool f32, int64_t status) {
   c10::cuda::CUDAGuard guard(x.device());
-  const bool grad = at::GradMode::is_enabled();
-  return Linear::apply(x, weight, wc, ws, tc, ts, f32, grad && x.requires_grad(),
-                       grad && weight.has_value() && weight->requires_grad(), status);
+  const bool grad = at::GradMode::is_enabled(), need_x = grad && x.requires_grad();
+  const bool need_w = grad && weight.has_value() && weight->requires_grad();
+  if (need_x || need_w) return Linear::apply(x, weight, wc, ws, tc, ts, f32, need_x, need_w, status);
+  at::NoGradGuard no_grad;
+  const Held w = weight.has_value() ? quantize_rows(rows_of(*weight), true, kRows).first : Held{*wc, *ws};
+  const Tensor y = product(quantize_rows(rows_of(x), false, kRows).first, in_place(w), true, f32,
+                           reinterpret_cast<uint32_t*>(status), Tensor());
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = y.size(1);
+  return y.view(shape);
 }
 
 struct NormOut {
@@ -225,7 +231,6 @@ struct Norm : torch::autograd::Function<Norm> {
     const Tensor x2 = rows_of(x), w = weight.contiguous();
     const NormOut o = norm_forward(x2, w, residual.has_value() ? rows_of(*residual) : Tensor(), eps, false, true);
     ctx->save_for_backward({o.h.defined() ? o.h : x2, w, o.rstd});
-    ctx->saved_data["eps"] = eps;
     variable_list out{o.y.view(x.sizes())};
     if (o.h.defined()) out.push_back(o.h.view(x.sizes()));
     return out;
@@ -240,7 +245,7 @@ struct Norm : torch::autograd::Function<Norm> {
       return {dh, dh.defined() ? at::zeros_like(w) : Tensor(), dh, Tensor()};
     c10::cuda::CUDAGuard guard(h.device());
     const Tensor dx = at::empty(h.sizes(), h.options()), dw = at::empty_like(w);
-    const race_norm_desc_t d{code_of(h), code_of(w), h.size(0), h.size(1), (float)ctx->saved_data["eps"].toDouble()};
+    const race_norm_desc_t d{code_of(h), code_of(w), h.size(0), h.size(1), 0.f};   // rstd has eps in it
     const size_t need = race_rms_norm_workspace(&d);
     const Tensor ws = at::empty({(int64_t)std::max<size_t>(need, 16)}, h.options().dtype(at::kByte));
     check(race_rms_norm_backward(&d, rr(rows_of(dy)), dh.defined() ? rr(rows_of(dh)) : rr(dh), rr(h), w.data_ptr(),
