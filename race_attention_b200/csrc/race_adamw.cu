@@ -430,7 +430,8 @@ extern "C" int race_adamw(const race_adamw_desc_t* desc, const race_adamw_tensor
     return RACE_ERR_INVALID;
   for (int64_t i = 0; i < count; ++i) {
     const race_adamw_tensor_t& t = tensors[i];
-    if (t.numel < 0 || t.step < 0 || t.first % 8 != 0 || (t.dtype != RACE_F32 && t.dtype != RACE_BF16)) return RACE_ERR_INVALID;
+    if (t.numel < 0 || t.step < 0 || t.first % 8 != 0 || (t.dtype != RACE_F32 && t.dtype != RACE_BF16))
+      return RACE_ERR_INVALID;
     if (t.numel == 0) continue;
     if (t.param == nullptr || t.grad == nullptr || t.exp_avg == nullptr || t.exp_avg_sq == nullptr)
       return RACE_ERR_INVALID;

@@ -23,15 +23,18 @@
 // columns, in registers.  A block takes the tensor core 450 cycles (four
 // instructions of 112) and the promotion 420, most of it loads from tensor memory;
 // tensor memory holds two accumulators, so one block is promoted while the
-// next is multiplied.  What bounds it is the way round: a block's completion takes
-// about 300 cycles to be seen by the promoting warps of both CTAs, the second
-// CTA's arrival as long to come back, so a block takes 950.  Waits are four
-// instructions long because each stands in that way.  Measured, 16384 x 8192 x 4096:
-// 501 us from a cold start (2193 TFLOP/s, 1965 MHz), 580 us kept up (1897,
-// 1485 MHz under the 1000 W cap); k_mm_split takes 1551 there.  Sixteen promoting
+// next is multiplied.  The way round takes 950 cycles a block: its completion is
+// seen by the promoting warps of both CTAs some 300 cycles later, and the second
+// CTA's arrival takes as long to come back; waits are four instructions long
+// because each stands in that way.  At full load the power cap is the bound, at
+// six blocks a tile too: 16384 x 8192 x 4096 takes 501 us from a cold start (2193 TFLOP/s,
+// 1965 MHz) and 575 kept up (1910, 1480 MHz, 990 W), 65536 x 2304 x 768 162 us (1435,
+// 1680 MHz, 1000 W); one 128 x 128 tile a CTA took 1551 for the first.  Sixteen promoting
 // warps took 637 (they share the schedulers with the issuing warp), halves of 128
-// columns with four accumulators 869 (twice the waits).  Results leave through
-// shared memory by TMA, 128 bytes of a row at a time.
+// columns with four accumulators 869, with an issuing warp each 535.  Where b has a
+// scale for each row (dw) an element takes two multiplications in place of one, and
+// promotion is the bound: 4736 x 4096 x 8192 231 us, with square blocks 159.  Results
+// leave through shared memory by TMA, 128 bytes of a row at a time.
 #include <atomic>
 
 #include "race_api.h"
