@@ -180,7 +180,7 @@ struct Split {
   static constexpr int RED = NT * 128 * 4;                         // joined partial tile
   static constexpr int SCALES = S * STAGE;                         // [2][NT] floats
   static constexpr int BARS = SCALES + 2 * NT * 4;                 // full, empty [S]; tfull, tempty [2]; drain
-  static constexpr int MISC = BARS + (2 * S + 5) * 8;              // tmem base, abort word
+  static constexpr int MISC = BARS + (2 * S + 5) * 8;              // tmem base, abort word, work that stays in flight
   static constexpr int BYTES = MISC + 16 + 1024;                   // + alignment
   static constexpr int COLS = 2 * NT < 32 ? 32 : 2 * NT;
   // Few tokens: a launch takes 4 us and its preparation one of them, which runs
@@ -224,6 +224,7 @@ __global__ void __launch_bounds__(kSplitThreads)
     }
     bar_init(drain);                                               // + the fence for all
     *abort = 0;
+    misc[2] = 0;
   }
   if (warp == 1) t5::tmem_alloc<L::COLS>(misc);
   fence_before();
@@ -238,13 +239,13 @@ __global__ void __launch_bounds__(kSplitThreads)
   const uint32_t tm = misc[0];
   const uint32_t full0 = saddr(full), empty0 = saddr(empty);
   float* red = reinterpret_cast<float*>(sm);                       // [NT][128]
+  int loaded = 0;                                                  // blocks whose copies warp 0 has issued
 
   if (warp == 0) {
     const uint32_t dst = saddr(sm);
-    int i = 0;
     bool ok = true;
-    for (; i < blocks; ++i) {
-      const int s = i % L::S;
+    for (; loaded < blocks; ++loaded) {
+      const int i = loaded, s = i % L::S;
       if (i >= L::S) ok = wait(empty0 + 8 * s, ((i / L::S) - 1) & 1, abort, a.polls);
       if (!__all_sync(0xffffffffu, ok)) break;
       if (elect()) {
@@ -254,13 +255,9 @@ __global__ void __launch_bounds__(kSplitThreads)
       }
       __syncwarp();
     }
-    const int from = i > L::S ? i - L::S : 0;
-    if (i < blocks) {                                              // gave up: copies in flight land first
-      for (int j = from; j < i; ++j)
-        if (!bar_wait(full + j % L::S, (j / L::S) & 1) && lane == 0) report(a.status, t5::kErrStuck);
-    } else {                                                       // the last commits have arrived
-      for (int j = from; j < i && ok; ++j) ok = wait(empty0 + 8 * (j % L::S), (j / L::S) & 1, abort, a.polls);
-    }
+    // the last commits reach this CTA's barriers before it leaves
+    for (int j = loaded > L::S ? loaded - L::S : 0; ok && j < loaded; ++j)
+      ok = wait(empty0 + 8 * (j % L::S), (j / L::S) & 1, abort, a.polls);
   } else if (warp == 1) {
     const uint64_t da = t5::desc_sw128(sm, 0), db = t5::desc_sw128(sm + L::A, 0);
     const uint32_t tempty0 = saddr(tempty);
@@ -339,8 +336,16 @@ __global__ void __launch_bounds__(kSplitThreads)
     for (int j = 0; j < NT; ++j) red[j * 128 + row] = acc[j];
   }
   __syncthreads();
-  const bool failed = *abort != 0;
-  if (failed && tid == 0) report(a.status, t5::kErrTimeout);
+  const bool failed = *abort != 0;                                 // final: every role has ended
+  if (failed) {
+    // A wait ran out, this warp's own or another's: its copies land before the
+    // shared memory that they go to is given back.
+    if (warp == 0)
+      for (int j = loaded > L::S ? loaded - L::S : 0; j < loaded; ++j)
+        if (!bar_wait(full + j % L::S, (j / L::S) & 1)) misc[2] = 1;
+    __syncthreads();
+    if (tid == 0) report(a.status, t5::kErrTimeout | (misc[2] != 0 ? t5::kErrStuck : 0));
+  }
   if (warp == 1) t5::tmem_free<L::COLS>(tm);
   if (C > 1) cluster_sync();
   // The ranks share the tile's tokens; a thread joins four weight rows of one,
