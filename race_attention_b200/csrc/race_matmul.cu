@@ -173,6 +173,18 @@ __device__ __forceinline__ void report(unsigned* status, unsigned bits) {
   __threadfence_system();
 }
 
+// Waits, after a launch has given up and its instructions are done, for the arrivals
+// of the last blocks' commits, in their order.
+template <int S>
+__device__ __forceinline__ bool settled(int sent, uint64_t* empty, uint64_t* tfull) {
+  bool ok = true;
+  for (int j = sent > S ? sent - S : 0; j < sent; ++j) {
+    ok &= bar_wait(empty + j % S, (j / S) & 1);
+    ok &= bar_wait(tfull + (j & 1), (j >> 1) & 1);
+  }
+  return ok;
+}
+
 template <int NT>
 struct Split {
   static constexpr int A = 128 * 128, B = NT * 128, STAGE = A + B;
@@ -239,13 +251,13 @@ __global__ void __launch_bounds__(kSplitThreads)
   const uint32_t tm = misc[0];
   const uint32_t full0 = saddr(full), empty0 = saddr(empty);
   float* red = reinterpret_cast<float*>(sm);                       // [NT][128]
-  int loaded = 0;                                                  // blocks whose copies warp 0 has issued
+  int sent = 0;                                                    // blocks whose copies (warp 0) or instructions (warp 1) are issued
 
   if (warp == 0) {
     const uint32_t dst = saddr(sm);
     bool ok = true;
-    for (; loaded < blocks; ++loaded) {
-      const int i = loaded, s = i % L::S;
+    for (; sent < blocks; ++sent) {
+      const int i = sent, s = i % L::S;
       if (i >= L::S) ok = wait(empty0 + 8 * s, ((i / L::S) - 1) & 1, abort, a.polls);
       if (!__all_sync(0xffffffffu, ok)) break;
       if (elect()) {
@@ -256,14 +268,13 @@ __global__ void __launch_bounds__(kSplitThreads)
       __syncwarp();
     }
     // the last commits reach this CTA's barriers before it leaves
-    for (int j = loaded > L::S ? loaded - L::S : 0; ok && j < loaded; ++j)
+    for (int j = sent > L::S ? sent - L::S : 0; ok && j < sent; ++j)
       ok = wait(empty0 + 8 * (j % L::S), (j / L::S) & 1, abort, a.polls);
   } else if (warp == 1) {
     const uint64_t da = t5::desc_sw128(sm, 0), db = t5::desc_sw128(sm + L::A, 0);
     const uint32_t tempty0 = saddr(tempty);
-    int i = 0;
-    for (; i < blocks; ++i) {
-      const int s = i % L::S, b = i & 1;
+    for (; sent < blocks; ++sent) {
+      const int i = sent, s = i % L::S, b = i & 1;
       const bool ok = wait(full0 + 8 * s, (i / L::S) & 1, abort, a.polls) &&
                       (i < 2 || wait(tempty0 + 8 * b, ((i >> 1) - 1) & 1, abort, a.polls));
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -277,11 +288,6 @@ __global__ void __launch_bounds__(kSplitThreads)
         t5::commit(empty + s);
       }
       __syncwarp();
-    }
-    if (i < blocks) {
-      if (elect()) t5::commit(drain);
-      __syncwarp();
-      if (!bar_wait(drain, 0) && lane == 0) report(a.status, t5::kErrStuck);
     }
   } else {
     // row of the tile (weight row) = tensor-memory lane; columns = tokens
@@ -338,11 +344,18 @@ __global__ void __launch_bounds__(kSplitThreads)
   __syncthreads();
   const bool failed = *abort != 0;                                 // final: every role has ended
   if (failed) {
-    // A wait ran out, this warp's own or another's: its copies land before the
-    // shared memory that they go to is given back.
-    if (warp == 0)
-      for (int j = loaded > L::S ? loaded - L::S : 0; j < loaded; ++j)
-        if (!bar_wait(full + j % L::S, (j / L::S) & 1)) misc[2] = 1;
+    // A wait ran out, this role's own or another's.  What is in flight ends before
+    // the memory that it reaches is given back: the copies, then the instructions
+    // (the lane that issued them commits once more) and their arrivals.
+    bool ok = true;
+    if (warp == 0) {
+      for (int j = sent > L::S ? sent - L::S : 0; j < sent; ++j) ok &= bar_wait(full + j % L::S, (j / L::S) & 1);
+    } else if (warp == 1) {
+      if (elect()) t5::commit(drain);
+      __syncwarp();
+      ok = bar_wait(drain, 0) && settled<L::S>(sent, empty, tfull);
+    }
+    if (!ok) misc[2] = 1;
     __syncthreads();
     if (tid == 0) report(a.status, t5::kErrTimeout | (misc[2] != 0 ? t5::kErrStuck : 0));
   }
@@ -454,8 +467,8 @@ struct Pair {
   static constexpr int OUT = S * STAGE;                            // [8 warps][2] boxes of 32 x 128 bytes
   static constexpr int SCALES = OUT + 16 * 4096;                   // rows of b: [8 warps][2][128] floats
   static constexpr int BARS = SCALES + (SQ ? 0 : 8192);            // full, empty [S]; tfull, tempty [2]; drain
-  static constexpr int MISC = BARS + (2 * S + 5) * 8;              // tmem base, abort word, loads issued
-  static constexpr int BYTES = MISC + 16 + 1024;
+  static constexpr int MISC = BARS + (2 * S + 5) * 8;              // tmem base, abort word, blocks loaded, blocks multiplied,
+  static constexpr int BYTES = MISC + 32 + 1024;                   // work that stays in flight
   static_assert(BYTES <= 232448, "227 KB of shared memory");
 };
 
@@ -558,6 +571,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     bar_init(drain);
     misc[1] = 0;
     misc[2] = 0;
+    misc[3] = 0;
+    misc[4] = 0;
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(misc)));
@@ -632,11 +647,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         ok = __all_sync(0xffffffffu, ok);
       }
-      if (!ok) {
-        if (elect()) commit_pair(drain);
-        __syncwarp();
-        if (!bar_wait(drain, 0) && lane == 0) report(a.status, t5::kErrStuck);
-      }
+      if (lane == 0) misc[3] = it;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
@@ -828,25 +839,37 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
   __syncthreads();
   cluster_sync();
+  // Every role of both CTAs has ended.  Where a wait of either ran out, what is in
+  // flight ends before one of them leaves or gives memory back.
   const bool mine = *abort != 0;
-  if (mine && tid == 0) report(a.status, t5::kErrTimeout);
-  // Copies in flight land before either CTA leaves: the first CTA's barriers
-  // count both CTAs' bytes, so it settles what only one of them issued.
   const uint32_t other = ld_cluster_u32(map_rank(saddr(misc + 1), rank ^ 1));
-  if (rank == 0 && tid == 0 && (mine || other != 0)) {
-    const int i0 = (int)misc[2], i1 = (int)ld_cluster_u32(map_rank(saddr(misc + 2), 1));
-    const int lo = min(i0, i1), hi = max(i0, i1);
-    for (int j = lo; j < hi; ++j) {
-      uint64_t* f = full + j % L::S;
-      if (j < i0)
-        asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(saddr(f)),
-                     "r"(L::STAGE)
-                     : "memory");
-      else
-        bar_expect_tx(f, L::STAGE);
+  if (mine || other != 0) {                                        // the same for the pair
+    bool ok = true;
+    if (warp == 0 && rank == 0 && lane == 0) {
+      // the copies: the first CTA's barriers count both CTAs' bytes, so it settles
+      // what only one of them issued
+      const int i0 = (int)misc[2], i1 = (int)ld_cluster_u32(map_rank(saddr(misc + 2), 1));
+      const int lo = min(i0, i1), hi = max(i0, i1);
+      for (int j = lo; j < hi; ++j) {
+        uint64_t* f = full + j % L::S;
+        if (j < i0)
+          asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(saddr(f)),
+                       "r"(L::STAGE)
+                       : "memory");
+        else
+          bar_expect_tx(f, L::STAGE);
+      }
+      for (int j = hi > L::S ? hi - L::S : 0; j < hi; ++j) ok &= bar_wait(full + j % L::S, (j / L::S) & 1);
+    } else if (warp == 1) {
+      // the instructions (the lane that issued them commits once more) and their
+      // arrivals at both CTAs' barriers
+      if (rank == 0 && elect()) commit_pair(drain);
+      __syncwarp();
+      ok = bar_wait(drain, 0) && settled<L::S>((int)ld_cluster_u32(map_rank(saddr(misc + 3), 0)), empty, tfull);
     }
-    for (int j = hi > L::S ? hi - L::S : 0; j < hi; ++j)
-      if (!bar_wait(full + j % L::S, (j / L::S) & 1)) report(a.status, t5::kErrStuck);
+    if (!ok) misc[4] = 1;
+    __syncthreads();
+    if (tid == 0) report(a.status, (mine ? t5::kErrTimeout : 0) | (misc[4] != 0 ? t5::kErrStuck : 0));
   }
   __syncthreads();
   cluster_sync();

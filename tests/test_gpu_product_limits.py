@@ -57,3 +57,22 @@ def test_copies_land_before_the_kernel_leaves(m, n, k, polls):
         assert bits in (0, _lib.RACE_DEV_TIMEOUT)
         assert bits or polls > 1             # one poll is over long before a copy has landed
         assert torch.equal(fp8_matmul(a, b), ref)
+
+
+@pytest.mark.parametrize("polls", [1, 8, 48])
+@pytest.mark.parametrize("square", [True, False], ids=["square", "rows"])
+@pytest.mark.parametrize("m,n,k", [
+    (20000, 2304, 256),      # pairs of CTAs, tiles of two blocks, fewer than there are stages
+    (4096, 2304, 768),       # several tiles a pair
+    (2304, 768, 20000)])     # a contraction that is cut
+def test_instructions_end_before_a_pair_leaves(m, n, k, square, polls):
+    from race_attention_b200 import _lib
+    from race_attention_b200.fp8 import fp8_matmul
+    a, b = held(m, k, 3, False), held(n, k, 4, square)
+    ref = fp8_matmul(a, b)
+    assert _lib.last_kernels()[0] == "mm_pair"
+    for _ in range(5):
+        bits = limited(a, b, polls)
+        assert bits in (0, _lib.RACE_DEV_TIMEOUT)
+        assert bits or polls > 1
+        assert torch.equal(fp8_matmul(a, b), ref)
