@@ -174,13 +174,14 @@ __device__ __forceinline__ void report(unsigned* status, unsigned bits) {
 }
 
 // Waits, after a launch has given up and its instructions are done, for the arrivals
-// of the last blocks' commits, in their order.
+// of each barrier's last commit (the parity of an earlier one would be mistaken for
+// a phase that never comes).
 template <int S>
 __device__ __forceinline__ bool settled(int sent, uint64_t* empty, uint64_t* tfull) {
   bool ok = true;
   for (int j = sent > S ? sent - S : 0; j < sent; ++j) {
     ok &= bar_wait(empty + j % S, (j / S) & 1);
-    ok &= bar_wait(tfull + (j & 1), (j >> 1) & 1);
+    if (j >= sent - 2) ok &= bar_wait(tfull + (j & 1), (j >> 1) & 1);
   }
   return ok;
 }
