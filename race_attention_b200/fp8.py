@@ -124,6 +124,18 @@ def fp8_matmul(a: BlockFp8, b: BlockFp8, out_dtype: torch.dtype = torch.bfloat16
                        out, host_status.word(codes.device))
 
 
+def _check_pair(w: BlockFp8, t: BlockFp8) -> None:
+    """t as the transpose of the held weight w: what can be seen without reading the codes."""
+    c, d = w.codes, t.codes
+    n, k = c.shape
+    if not t.square or d.device != c.device or d.shape != (k, n):
+        raise ValueError(f"the transpose that goes with a held weight [{n}, {k}] needs square blocks, "
+                         f"[{k}, {n}], on the weight's device")
+    if n > 1 and d.data_ptr() == c.data_ptr() and d.stride() == c.stride():
+        raise ValueError("the weight itself stands in its transpose's place: "
+                         "quantize_fp8(w, square=True, transposed=True) returns both")
+
+
 Weight = Union[torch.Tensor, BlockFp8, Tuple[BlockFp8, BlockFp8]]
 
 
@@ -144,9 +156,14 @@ def fp8_linear(x: Union[torch.Tensor, BlockFp8], weight: Weight,
 
     out_dtype: float32 or bfloat16; by default x's type (bfloat16 where x comes
     in 8 bits)."""
-    held = weight if isinstance(weight, tuple) else (weight, None)
-    if not isinstance(held[0], BlockFp8):
-        held = None
+    held = None
+    if isinstance(weight, BlockFp8):
+        held = (weight, None)
+    elif not isinstance(weight, torch.Tensor):
+        if len(weight) != 2 or not all(isinstance(b, BlockFp8) for b in weight):
+            raise ValueError("weight must be a tensor, a BlockFp8, or the pair of a BlockFp8 and its transpose")
+        held = weight
+        _check_pair(*held)
     if isinstance(x, BlockFp8):
         if held is None:
             if torch.is_grad_enabled() and weight.requires_grad:
