@@ -331,7 +331,9 @@ int race_forward_static(const race_desc_t* desc, race_tensor_t q, race_tensor_t 
  * x * (1 / s) rounded to nearest even (each step in float32); a block that holds an infinity or a NaN
  * gets a non-finite scale, so that everything it enters shows it. */
 
-/* Rows of elements; `ld` elements between rows, columns contiguous. */
+/* Rows of elements; `ld` elements between rows, columns contiguous.  Here and below
+ * a pointer lies on a multiple of its element's size, codes, optimizer states and workspaces
+ * on 16 bytes; anything else is refused with RACE_ERR_ALIGN. */
 typedef struct {
   void* data;
   int64_t ld;

@@ -439,7 +439,8 @@ extern "C" int race_adamw(const race_adamw_desc_t* desc, const race_adamw_tensor
       return RACE_ERR_INVALID;
     const int es = t.dtype == RACE_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(t.param) % es != 0 || reinterpret_cast<uintptr_t>(t.grad) % es != 0 ||
-        reinterpret_cast<uintptr_t>(t.exp_avg) % 16 != 0 || reinterpret_cast<uintptr_t>(t.exp_avg_sq) % 16 != 0)
+        reinterpret_cast<uintptr_t>(t.exp_avg) % 16 != 0 || reinterpret_cast<uintptr_t>(t.exp_avg_sq) % 16 != 0 ||
+        (desc->state_bits == 8 && (!api_aligned(t.exp_avg_scale, 4) || !api_aligned(t.exp_avg_sq_scale, 4))))
       return RACE_ERR_ALIGN;
   }
   if (count == 0) return RACE_OK;

@@ -31,6 +31,9 @@ struct ApiCall {
 bool api_encode_bytes(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld,
                       int box_rows);
 
+// p lies on a multiple of `bytes` (a null pointer does)
+inline bool api_aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
 #define RACE_CALL(x)                 \
   do {                               \
     const int rc_ = (x);             \

@@ -996,8 +996,7 @@ int check(const race_matmul_desc_t* d) {
 
 int check_operand(race_blocks_t b, int64_t rows, int64_t k) {
   if (b.codes == nullptr || b.scales == nullptr) return RACE_ERR_INVALID;
-  if (reinterpret_cast<uintptr_t>(b.codes) % 16 != 0 || b.ld % 16 != 0 || b.ld <= 0)
-    return RACE_ERR_ALIGN;
+  if (!api_aligned(b.codes, 16) || b.ld % 16 != 0 || b.ld <= 0 || !api_aligned(b.scales, 4)) return RACE_ERR_ALIGN;
   return b.ld >= k || rows <= 1 ? RACE_OK : RACE_ERR_INVALID;
 }
 
@@ -1020,15 +1019,18 @@ extern "C" int race_scaled_matmul(const race_matmul_desc_t* desc, race_blocks_t 
   if (desc->m == 0 || desc->n == 0) return RACE_OK;
   const int es = desc->out_dtype == RACE_F32 ? 4 : 2;
   if (result.data == nullptr || (desc->m > 1 && result.ld < desc->n)) return RACE_ERR_INVALID;
-  if (reinterpret_cast<uintptr_t>(result.data) % es != 0) return RACE_ERR_ALIGN;
+  if (!api_aligned(result.data, es) || !api_aligned(status, 4)) return RACE_ERR_ALIGN;
+  if (desc->k > 0) {
+    RACE_CALL(mm::check_operand(a, desc->m, desc->k));
+    RACE_CALL(mm::check_operand(b, desc->n, desc->k));
+    if (!api_aligned(workspace, 16)) return RACE_ERR_ALIGN;          // partial results are read four at a time
+  }
   RACE_CALL(api_bind(stream));
   if (desc->k == 0) {   // an empty sum
     const cudaError_t e = cudaMemset2DAsync(result.data, (size_t)(desc->m > 1 ? result.ld : desc->n) * es, 0,
                                             (size_t)desc->n * es, (size_t)desc->m, stream);
     return e == cudaSuccess ? RACE_OK : api_cuda_fail(e);
   }
-  RACE_CALL(mm::check_operand(a, desc->m, desc->k));
-  RACE_CALL(mm::check_operand(b, desc->n, desc->k));
   mm::Args g{a.scales, a.stride_row, a.stride_block, b.scales, b.stride_row, b.stride_block,
              result.data, result.ld, desc->out_dtype == RACE_BF16, desc->m, desc->n,
              (int)((desc->k + 127) / 128), 1, desc->wait_polls > 0 ? desc->wait_polls : mm::kPolls, status};

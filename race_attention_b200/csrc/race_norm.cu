@@ -615,12 +615,13 @@ extern "C" int race_rms_norm(const race_norm_desc_t* desc, race_rows_t x, race_r
   RACE_CALL(norm::check_rows(desc, residual, false));
   RACE_CALL(norm::check_rows(desc, y, false));
   RACE_CALL(norm::check_rows(desc, h, residual.data != nullptr));
+  if (!api_aligned(weight, desc->weight_dtype == RACE_F32 ? 4 : 2) || !api_aligned(rstd, 4)) return RACE_ERR_ALIGN;
   if ((y.data != nullptr && y.ld < desc->width && desc->rows > 1) ||
       (residual.data != nullptr && h.ld < desc->width && desc->rows > 1))
     return RACE_ERR_INVALID;                 // results may not overlap
   if (y8.codes != nullptr) {
     if (y8.scales == nullptr) return RACE_ERR_INVALID;
-    if (reinterpret_cast<uintptr_t>(y8.codes) % 16 != 0 || y8.ld % 16 != 0) return RACE_ERR_ALIGN;
+    if (!api_aligned(y8.codes, 16) || y8.ld % 16 != 0 || !api_aligned(y8.scales, 4)) return RACE_ERR_ALIGN;
     if (y8.ld < desc->width) return RACE_ERR_INVALID;
   }
   RACE_CALL(api_bind(stream));
@@ -661,6 +662,9 @@ extern "C" int race_rms_norm_backward(const race_norm_desc_t* desc, race_rows_t 
   RACE_CALL(norm::check_rows(desc, dh, false));
   RACE_CALL(norm::check_rows(desc, h, any));
   RACE_CALL(norm::check_rows(desc, dx, any));
+  const int ws = desc->weight_dtype == RACE_F32 ? 4 : 2;
+  if (!api_aligned(weight, ws) || !api_aligned(dweight, ws) || !api_aligned(rstd, 4) || !api_aligned(workspace, 16))
+    return RACE_ERR_ALIGN;
   if (desc->rows > 1 && dx.ld < desc->width) return RACE_ERR_INVALID;
   RACE_CALL(api_bind(stream));
   const int wb = desc->weight_dtype == RACE_BF16;

@@ -263,7 +263,7 @@ void launch(const Args& a, bool square, cudaStream_t s) {
 int check_blocks(race_blocks_t b, int64_t cols, bool scales) {
   if (b.codes == nullptr) return RACE_OK;
   if (scales && b.scales == nullptr) return RACE_ERR_INVALID;
-  if (reinterpret_cast<uintptr_t>(b.codes) % 16 != 0 || b.ld % 16 != 0) return RACE_ERR_ALIGN;
+  if (!api_aligned(b.codes, 16) || b.ld % 16 != 0 || !api_aligned(b.scales, 4)) return RACE_ERR_ALIGN;
   return b.ld >= cols ? RACE_OK : RACE_ERR_INVALID;
 }
 
