@@ -434,7 +434,8 @@ typedef struct {
 /* p -= lr * weight_decay * p; m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g^2;
  * p -= lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps), t = step + 1, for every
  * tensor of the list (a host array; it is passed to the kernels by value, so
- * it may be freed on return).  bfloat16 parameters and 8-bit states are
+ * it may be freed on return; the step's count, rate and noise go with it, and a stream
+ * that is being captured is refused, RACE_ERR_UNSUPPORTED).  bfloat16 parameters and 8-bit states are
  * rounded up or down with the probability of the part cut off, by noise that
  * is a function of seed, t and the element's index alone. */
 int race_adamw(const race_adamw_desc_t* desc, const race_adamw_tensor_t* tensors, int64_t count,

@@ -9,8 +9,9 @@
 // states 16.1 (266 us, 5.8 TB/s).  bfloat16 with 8-bit states moves 10.1 and is bound by
 // its 90 instructions a parameter, half of them logic (184 M: 514 us, 3.6 TB/s).  The tensors'
 // addresses travel in the kernel's parameters (up to 384 tensors in the 32 KB
-// that a launch carries), so a step needs no copy to the device and can be
-// captured; a CTA finds its 2048 elements by bisection over the running chunk
+// that a launch carries), so a step needs no copy to the device; the step's count,
+// learning rate and noise travel with them, which is why a capture is refused: each
+// replay would repeat them.  A CTA finds its 2048 elements by bisection over the running chunk
 // counts.  A thread holds 8 consecutive elements, half a warp one 128-element
 // block of the states.
 //
@@ -444,7 +445,12 @@ extern "C" int race_adamw(const race_adamw_desc_t* desc, const race_adamw_tensor
       return RACE_ERR_ALIGN;
   }
   if (count == 0) return RACE_OK;
-  RACE_CALL(api_bind(stream));
+  bool capturing = false;
+  RACE_CALL(api_bind(stream, &capturing));
+  if (capturing) {
+    api_note("adamw: a graph would repeat this step's count, learning rate and noise; call it outside the capture");
+    return RACE_ERR_UNSUPPORTED;
+  }
   // 32-bit states take both types in one launch, 8-bit states one after the other
   for (int type = 0; type < (desc->state_bits == 8 ? 2 : 1); ++type) {
     int64_t pick[adamw::kMany];

@@ -12,7 +12,8 @@ namespace race {
 
 void api_begin();
 void api_end();
-int api_bind(cudaStream_t stream);            // makes the stream's device current
+// Makes the stream's device current; *capturing: whether the stream is being captured.
+int api_bind(cudaStream_t stream, bool* capturing = nullptr);
 int api_cuda_fail(cudaError_t e);             // records the text, returns RACE_ERR_CUDA
 void api_log(const char* kernel);             // adds a launch to race_last_kernels()
 int api_sm_count();

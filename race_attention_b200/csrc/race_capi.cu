@@ -579,12 +579,13 @@ bool encode_map3(CUtensorMap* m, const float* base, int64_t N, int64_t T, int C,
 
 void api_begin() { new_scope(); }
 void api_end() { end_scope(); }
-int api_bind(cudaStream_t stream) {
+int api_bind(cudaStream_t stream, bool* capturing) {
   // A stream's device cannot be asked for while it is being captured; the
   // capturing thread has its context current.
   cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
   const cudaError_t e = cudaStreamIsCapturing(stream, &st);
   if (e != cudaSuccess) return cuda_fail(e);
+  if (capturing != nullptr) *capturing = st != cudaStreamCaptureStatusNone;
   return st == cudaStreamCaptureStatusNone ? bind_device(stream) : RACE_OK;
 }
 int api_cuda_fail(cudaError_t e) { return cuda_fail(e); }

@@ -13,7 +13,7 @@ block.  A block that holds an infinity or a NaN gets a non-finite scale.
 
 All calls run on the current stream of the inputs' device, allocate through
 torch's caching allocator, never synchronise and can be captured in a CUDA graph
-(after a first call outside the capture).
+(after a first call outside the capture); the optimizer's step cannot.
 """
 from __future__ import annotations
 

@@ -28,6 +28,9 @@ class AdamW(torch.optim.Optimizer):
       the format are not lost; a second moment above zero is never held as zero.
     seed: of that rounding; equal seeds and equal inputs give equal results.
 
+    A step takes its count, learning rate and noise from the host, so it is refused
+    while a CUDA graph is being captured: capture the passes before it alone.
+
     ``exp_avg``, ``exp_avg_sq`` and, with 8 bits, ``exp_avg_scale`` and
     ``exp_avg_sq_scale`` are the states of all parameters (``offsets`` says
     where each begins); with 8 bits ``exp_avg_sq`` holds the codes of sqrt(v)."""
