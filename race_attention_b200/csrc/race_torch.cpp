@@ -75,6 +75,9 @@ race_blocks_t rb(const Held& h) {
                        h.scales.stride(1)};
 }
 
+// Autograd's version check has to see what a kernel wrote into a caller's tensor.
+void written(const Tensor& x) { x.unsafeGetTensorImpl()->bump_version(); }
+
 enum Mode { kRows = 0, kBoth = 1, kCols = 2 };
 
 std::pair<Held, Held> quantize_rows(const Tensor& x, bool square, int mode) {
@@ -136,8 +139,10 @@ Tensor matmul(const Tensor& ac, const Tensor& as, bool a_square, const Tensor& b
   }
   c10::cuda::CUDAGuard guard(ac.device());
   at::NoGradGuard no_grad;
-  return product(in_place({ac, as}), in_place({bc, bs}), b_square, f32, reinterpret_cast<uint32_t*>(status),
-                 out.has_value() ? *out : Tensor());
+  const Tensor y = product(in_place({ac, as}), in_place({bc, bs}), b_square, f32, reinterpret_cast<uint32_t*>(status),
+                           out.has_value() ? *out : Tensor());
+  if (out.has_value()) written(y);
+  return y;
 }
 
 // The gradients are computed outside torch, so they have none of their own.
@@ -281,7 +286,7 @@ void adamw(const std::vector<Tensor>& params, const std::vector<int64_t>& first,
   c10::cuda::CUDAGuard guard(m.device());
   at::NoGradGuard no_grad;
   std::vector<race_adamw_tensor_t> table;
-  std::vector<int32_t*> moved;
+  std::vector<size_t> moved;
   std::vector<Tensor> kept;
   table.reserve(params.size());
   moved.reserve(params.size());
@@ -307,11 +312,14 @@ void adamw(const std::vector<Tensor>& params, const std::vector<int64_t>& first,
     table.push_back({p.data_ptr(), g.data_ptr(), mp + at * size, vp + at * size, msp ? msp + at / kBlock : nullptr,
                      vsp ? vsp + at / kBlock : nullptr, sizes[i], (uint64_t)at, t == at::kFloat ? RACE_F32 : RACE_BF16,
                      step[i]});
-    moved.push_back(step + i);
+    moved.push_back(i);
   }
   const race_adamw_desc_t d{lr, b1, b2, eps, decay, (uint32_t)seed, (int32_t)bits};
   check(race_adamw(&d, table.data(), (int64_t)table.size(), stream_of(m)));
-  for (int32_t* s : moved) ++*s;
+  for (const size_t i : moved) {
+    ++step[i];
+    written(params[i]);
+  }
 }
 
 }  // namespace

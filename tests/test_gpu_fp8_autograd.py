@@ -1,0 +1,47 @@
+"""The 8-bit operators beside torch's autograd (needs a B200): writes into a caller's
+tensor are seen by its version check."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from race_attention_b200 import _lib
+    _lib.load()
+
+
+def randn(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_step_between_the_passes_is_seen(bits):
+    from race_attention_b200.fp8 import rms_norm
+    from race_attention_b200.optim import AdamW
+    x, w, still = randn(4, 64), torch.nn.Parameter(torch.ones(64, device="cuda")), torch.nn.Parameter(randn(64))
+    opt = AdamW([w, still], state_bits=bits)
+    w.grad = torch.ones_like(w)
+    kept = still._version
+    y = rms_norm(x, w)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    assert still._version == kept           # it had no gradient and did not move
+    opt.zero_grad()
+    rms_norm(x, w).sum().backward()
+    assert w.grad is not None
+
+
+def test_a_product_into_a_saved_tensor_is_seen():
+    from race_attention_b200.fp8 import fp8_matmul, quantize_fp8
+    a, b = quantize_fp8(randn(8, 256)), quantize_fp8(randn(16, 256, seed=1))
+    out = torch.ones(8, 16, device="cuda")
+    x = randn(8, 16, seed=2).requires_grad_()
+    y = (x * out).sum()
+    assert fp8_matmul(a, b, torch.float32, out=out) is out
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
