@@ -150,6 +150,14 @@ void once() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "the 8-bit operators have no second derivatives (create_graph=True)");
 }
 
+bool has_tangent(const Tensor& x) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(/*level=*/0).defined();
+}
+// Calls that need no gradient skip the autograd functions, which would refuse a tangent.
+void no_tangent(const Tensor& x) {
+  TORCH_CHECK(!has_tangent(x), "the 8-bit operators have no forward-mode derivatives");
+}
+
 struct Linear : torch::autograd::Function<Linear> {
   // x [..., K]; weight [N, K], or none with its held form (codes, scales and those of its transpose)
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& weight, const Maybe& wc, const Maybe& ws,
@@ -195,6 +203,8 @@ struct Linear : torch::autograd::Function<Linear> {
 
 Tensor linear(const Tensor& x, const Maybe& weight, const Maybe& wc, const Maybe& ws, const Maybe& tc, const Maybe& ts,
               bool f32, int64_t status) {
+  no_tangent(x);
+  if (weight.has_value()) no_tangent(*weight);
   c10::cuda::CUDAGuard guard(x.device());
   const bool grad = at::GradMode::is_enabled(), need_x = grad && x.requires_grad();
   const bool need_w = grad && weight.has_value() && weight->requires_grad();
@@ -264,6 +274,9 @@ struct Norm : torch::autograd::Function<Norm> {
 // (y or codes, scales, h), the unused ones undefined
 std::tuple<Tensor, Tensor, Tensor> norm(const Tensor& x, const Tensor& weight, const Maybe& residual, double eps,
                                         bool quant, bool grad) {
+  no_tangent(x);
+  no_tangent(weight);
+  if (residual.has_value()) no_tangent(*residual);
   c10::cuda::CUDAGuard guard(x.device());
   if (grad) {
     const variable_list out = Norm::apply(x, weight, residual, eps);
@@ -338,4 +351,5 @@ PYBIND11_MODULE(_race_torch, m) {
   m.def("linear", &linear);
   m.def("norm", &norm);
   m.def("adamw", &adamw);
+  m.def("has_tangent", &has_tangent);
 }

@@ -166,7 +166,7 @@ def fp8_linear(x: Union[torch.Tensor, BlockFp8], weight: Weight,
         _check_pair(*held)
     if isinstance(x, BlockFp8):
         if held is None:
-            if torch.is_grad_enabled() and weight.requires_grad:
+            if (torch.is_grad_enabled() and weight.requires_grad) or _ops.has_tangent(weight):
                 raise ValueError("x in 8 bits has no gradient: pass the tensor itself to train")
             held = (quantize_fp8(weight, square=True), None)
         return fp8_matmul(x, held[0], torch.bfloat16 if out_dtype is None else out_dtype)

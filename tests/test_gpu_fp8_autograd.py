@@ -45,3 +45,25 @@ def test_a_product_into_a_saved_tensor_is_seen():
     assert fp8_matmul(a, b, torch.float32, out=out) is out
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_tangents_are_refused():
+    """Without an input that requires grad no autograd function stands in the way: the
+    call itself refuses, with gradients enabled or not."""
+    import torch.autograd.forward_ad as fw
+    from race_attention_b200.fp8 import fp8_linear, quantize_fp8, rms_norm
+    x, w, n = randn(8, 256), randn(96, 256, seed=1), torch.ones(256, device="cuda")
+    held = quantize_fp8(w, square=True)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda: fp8_linear(dual(x), w), lambda: fp8_linear(x, dual(w)), lambda: fp8_linear(dual(x), held),
+                 lambda: fp8_linear(dual(x).half(), w), lambda: rms_norm(dual(x), n), lambda: rms_norm(x, dual(n)),
+                 lambda: rms_norm(x, n, residual=dual(x)), lambda: rms_norm(dual(x), n, quantize=True),
+                 lambda: fp8_linear(dual(x).requires_grad_(), w)]
+        for f in calls:
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode|jvp"):
+                    f()
+        with pytest.raises(ValueError, match="no gradient"):
+            fp8_linear(quantize_fp8(x), dual(w))
+        assert fp8_linear(x, w).shape == (8, 96) and rms_norm(x, n).shape == x.shape    # nothing to lose here
