@@ -103,16 +103,31 @@ Held in_place(const Held& h) {
   return {n, h.scales};
 }
 
-Tensor product(const Held& a, const Held& b, bool square, bool f32, uint32_t* status, const Tensor& out_or_none) {
+// The product in `y` ([m, n], any row stride).
+void product_into(const Tensor& y, int64_t ld, const Held& a, const Held& b, bool square, bool f32, uint32_t* status) {
   const int64_t m = a.codes.size(0), n = b.codes.size(0), k = a.codes.size(1);
-  Tensor y = out_or_none.defined() ? out_or_none
-                                   : at::empty({m, n}, a.codes.options().dtype(f32 ? at::kFloat : at::kBFloat16));
   const race_matmul_desc_t d{f32 ? RACE_F32 : RACE_BF16, square, m, n, k, 0, 0};
   const size_t need = race_scaled_matmul_workspace(&d);
   Tensor ws;
   if (need > 0) ws = at::empty({(int64_t)need}, a.codes.options().dtype(at::kByte));
-  check(race_scaled_matmul(&d, rb(a), rb(b), rr(y), status, need > 0 ? ws.data_ptr() : nullptr, need, stream_of(y)));
+  check(race_scaled_matmul(&d, rb(a), rb(b), race_rows_t{y.data_ptr(), ld}, status, need > 0 ? ws.data_ptr() : nullptr,
+                           need, stream_of(y)));
+}
+
+// The product as a tensor of `shape`, whose last axis is n.  Results are allocated
+// with their shape: autograd refuses to change a view in place that an autograd
+// function has made.
+Tensor product(const Held& a, const Held& b, bool square, bool f32, uint32_t* status, at::IntArrayRef shape) {
+  const Tensor y = at::empty(shape, a.codes.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  product_into(y, b.codes.size(0), a, b, square, f32, status);
   return y;
+}
+
+// x's sizes with n in the place of the last one
+std::vector<int64_t> shape_of(const Tensor& x, int64_t n) {
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = n;
+  return shape;
 }
 
 // ------------------------------------------------------------------ entry points
@@ -139,10 +154,12 @@ Tensor matmul(const Tensor& ac, const Tensor& as, bool a_square, const Tensor& b
   }
   c10::cuda::CUDAGuard guard(ac.device());
   at::NoGradGuard no_grad;
-  const Tensor y = product(in_place({ac, as}), in_place({bc, bs}), b_square, f32, reinterpret_cast<uint32_t*>(status),
-                           out.has_value() ? *out : Tensor());
-  if (out.has_value()) written(y);
-  return y;
+  auto* word = reinterpret_cast<uint32_t*>(status);
+  const Held a = in_place({ac, as}), b = in_place({bc, bs});
+  if (!out.has_value()) return product(a, b, b_square, f32, word, {ac.size(0), bc.size(0)});
+  product_into(*out, out->stride(0), a, b, b_square, f32, word);
+  written(*out);
+  return *out;
 }
 
 // The gradients are computed outside torch, so they have none of their own.
@@ -166,9 +183,8 @@ struct Linear : torch::autograd::Function<Linear> {
     const auto [xr, xt] = quantize_rows(x2, false, need_w ? kBoth : kRows);
     Held w{wc.value_or(none), ws.value_or(none)}, t{tc.value_or(none), ts.value_or(none)};
     if (weight.has_value()) std::tie(w, t) = quantize_rows(rows_of(*weight), true, need_x ? kBoth : kRows);
-    Tensor y = product(xr, in_place(w), true, f32, reinterpret_cast<uint32_t*>(status), Tensor());
-    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
-    shape.back() = y.size(1);
+    const Tensor y = product(xr, in_place(w), true, f32, reinterpret_cast<uint32_t*>(status),
+                             shape_of(x, w.codes.size(0)));
     if (need_x || need_w) {
       ctx->save_for_backward({need_w ? xt.codes : Tensor(), need_w ? xt.scales : Tensor(),
                               need_x ? t.codes : Tensor(), need_x ? t.scales : Tensor()});
@@ -178,7 +194,7 @@ struct Linear : torch::autograd::Function<Linear> {
       meta.insert(meta.end(), x.sizes().begin(), x.sizes().end());
       ctx->saved_data["meta"] = meta;
     }
-    return y.view(shape);
+    return y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -192,10 +208,9 @@ struct Linear : torch::autograd::Function<Linear> {
       c10::cuda::CUDAGuard guard(grads[0].device());
       const auto [r, c] = quantize_rows(rows_of(grads[0]), false, need_x ? need_w ? kBoth : kRows : kCols);
       if (need_x)
-        dx = product(r, in_place({saved[2], saved[3]}), true, meta[1] != 0, status, Tensor())
-                 .view(at::IntArrayRef(meta).slice(5));
+        dx = product(r, in_place({saved[2], saved[3]}), true, meta[1] != 0, status, at::IntArrayRef(meta).slice(5));
       if (need_w)
-        dw = product(c, {saved[0], saved[1]}, false, meta[2] != 0, status, Tensor());
+        dw = product(c, {saved[0], saved[1]}, false, meta[2] != 0, status, {c.codes.size(0), saved[0].size(0)});
     }
     return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -211,11 +226,8 @@ Tensor linear(const Tensor& x, const Maybe& weight, const Maybe& wc, const Maybe
   if (need_x || need_w) return Linear::apply(x, weight, wc, ws, tc, ts, f32, need_x, need_w, status);
   at::NoGradGuard no_grad;
   const Held w = weight.has_value() ? quantize_rows(rows_of(*weight), true, kRows).first : Held{*wc, *ws};
-  const Tensor y = product(quantize_rows(rows_of(x), false, kRows).first, in_place(w), true, f32,
-                           reinterpret_cast<uint32_t*>(status), Tensor());
-  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
-  shape.back() = y.size(1);
-  return y.view(shape);
+  return product(quantize_rows(rows_of(x), false, kRows).first, in_place(w), true, f32,
+                 reinterpret_cast<uint32_t*>(status), shape_of(x, w.codes.size(0)));
 }
 
 struct NormOut {
@@ -223,18 +235,20 @@ struct NormOut {
   Held y8;
 };
 
+// x and residual as rows; y and h get `shape` (see product).
 NormOut norm_forward(const Tensor& x, const Tensor& weight, const Tensor& residual, double eps, bool quant,
-                     bool want_rstd) {
+                     bool want_rstd, at::IntArrayRef shape) {
   const int64_t r = x.size(0), k = x.size(1);
+  const auto whole = [k](const Tensor& t) { return race_rows_t{t.defined() ? t.data_ptr() : nullptr, k}; };
   NormOut o;
-  if (residual.defined()) o.h = at::empty({r, k}, x.options());
+  if (residual.defined()) o.h = at::empty(shape, x.options());
   if (quant)
     o.y8 = {new_codes(r, k, x), new_scales(r, k, x)};
   else
-    o.y = at::empty({r, k}, x.options());
+    o.y = at::empty(shape, x.options());
   if (want_rstd) o.rstd = at::empty({r}, x.options().dtype(at::kFloat));
   const race_norm_desc_t d{code_of(x), code_of(weight), r, k, (float)eps};
-  check(race_rms_norm(&d, rr(x), rr(residual), weight.data_ptr(), rr(o.y), rb(o.y8), rr(o.h),
+  check(race_rms_norm(&d, rr(x), rr(residual), weight.data_ptr(), whole(o.y), rb(o.y8), whole(o.h),
                       want_rstd ? static_cast<float*>(o.rstd.data_ptr()) : nullptr, stream_of(x)));
   return o;
 }
@@ -244,30 +258,30 @@ struct Norm : torch::autograd::Function<Norm> {
                                double eps) {
     ctx->set_materialize_grads(false);
     const Tensor x2 = rows_of(x), w = weight.contiguous();
-    const NormOut o = norm_forward(x2, w, residual.has_value() ? rows_of(*residual) : Tensor(), eps, false, true);
+    const NormOut o = norm_forward(x2, w, residual.has_value() ? rows_of(*residual) : Tensor(), eps, false, true,
+                                   x.sizes());
     ctx->save_for_backward({o.h.defined() ? o.h : x2, w, o.rstd});
-    variable_list out{o.y.view(x.sizes())};
-    if (o.h.defined()) out.push_back(o.h.view(x.sizes()));
+    variable_list out{o.y};
+    if (o.h.defined()) out.push_back(o.h);
     return out;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once();
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &h = saved[0], &w = saved[1], &rstd = saved[2];
+    const Tensor h = rows_of(saved[0]), &w = saved[1], &rstd = saved[2];
     const Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
     if (!dy.defined())   // y was not used: the norm passes dh through
       return {dh, dh.defined() ? at::zeros_like(w) : Tensor(), dh, Tensor()};
     c10::cuda::CUDAGuard guard(h.device());
-    const Tensor dx = at::empty(h.sizes(), h.options()), dw = at::empty_like(w);
+    const Tensor dx = at::empty(dy.sizes(), h.options()), dw = at::empty_like(w);
     const race_norm_desc_t d{code_of(h), code_of(w), h.size(0), h.size(1), 0.f};   // rstd has eps in it
     const size_t need = race_rms_norm_workspace(&d);
     const Tensor ws = at::empty({(int64_t)std::max<size_t>(need, 16)}, h.options().dtype(at::kByte));
     check(race_rms_norm_backward(&d, rr(rows_of(dy)), dh.defined() ? rr(rows_of(dh)) : rr(dh), rr(h), w.data_ptr(),
-                                 static_cast<const float*>(rstd.data_ptr()), rr(dx), dw.data_ptr(), ws.data_ptr(),
-                                 (size_t)ws.numel(), stream_of(h)));
-    const Tensor g = dx.view(dy.sizes());
-    return {g, dw, grads.size() > 1 ? g : Tensor(), Tensor()};
+                                 static_cast<const float*>(rstd.data_ptr()), race_rows_t{dx.data_ptr(), h.size(1)},
+                                 dw.data_ptr(), ws.data_ptr(), (size_t)ws.numel(), stream_of(h)));
+    return {dx, dw, grads.size() > 1 ? dx : Tensor(), Tensor()};
   }
 };
 
@@ -284,10 +298,9 @@ std::tuple<Tensor, Tensor, Tensor> norm(const Tensor& x, const Tensor& weight, c
   }
   at::NoGradGuard no_grad;
   const NormOut o = norm_forward(rows_of(x), weight.contiguous(), residual.has_value() ? rows_of(*residual) : Tensor(),
-                                 eps, quant, false);
-  const Tensor h = o.h.defined() ? o.h.view(x.sizes()) : o.h;
-  if (quant) return {o.y8.codes, o.y8.scales, h};
-  return {o.y.view(x.sizes()), Tensor(), h};
+                                 eps, quant, false, x.sizes());
+  if (quant) return {o.y8.codes, o.y8.scales, o.h};
+  return {o.y, Tensor(), o.h};
 }
 
 // One step of a parameter group.  first[i]: where parameter i's states begin;

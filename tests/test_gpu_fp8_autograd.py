@@ -67,3 +67,64 @@ def test_tangents_are_refused():
         with pytest.raises(ValueError, match="no gradient"):
             fp8_linear(quantize_fp8(x), dual(w))
         assert fp8_linear(x, w).shape == (8, 96) and rms_norm(x, n).shape == x.shape    # nothing to lose here
+
+
+@pytest.mark.parametrize("lead", [(6,), (2, 3), ()], ids=["rows", "axes", "vector"])
+def test_results_change_in_place(lead):
+    """y += b, an in-place activation and a slice's assignment, with the gradients of
+    the same steps out of place."""
+    from race_attention_b200.fp8 import fp8_linear, rms_norm
+    b = randn(96, seed=5)
+
+    def leaves():
+        return [t.requires_grad_() for t in (randn(*lead, 256), randn(96, 256, seed=1), 1 + 0.1 * randn(256, seed=2),
+                                             randn(*lead, 256, seed=3))]
+
+    def run(inplace):
+        x, w, n, r = leaves()
+        y, h = rms_norm(x, n, residual=r)
+        u = rms_norm(x, n)
+        if inplace:
+            y *= 0.5
+            torch.relu_(u)
+        else:
+            y, u = y * 0.5, torch.relu(u)
+        z = fp8_linear(y + u, w)
+        if inplace:
+            z += b
+            torch.nn.functional.relu(z, inplace=True)
+        else:
+            z = torch.relu(z + b)
+        return (z.detach(), *torch.autograd.grad((z, h), (x, w, n, r), (torch.ones_like(z), randn(*lead, 256, seed=4))))
+
+    for got, ref in zip(run(True), run(False)):
+        assert torch.equal(got, ref)
+
+
+def test_a_changed_residual_is_seen():
+    """The backward pass reads h, so it has to refuse one that changed."""
+    from race_attention_b200.fp8 import rms_norm
+    x, n = randn(4, 256).requires_grad_(), torch.ones(256, device="cuda")
+    y, h = rms_norm(x, n, residual=randn(4, 256, seed=1))
+    h += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        (y.sum() + h.sum()).backward()
+
+
+def test_results_hold_no_cycle():
+    """A result that is dropped frees its memory at once, the graph with it."""
+    import gc
+    from race_attention_b200.fp8 import fp8_linear, rms_norm
+    x, w, n = randn(512, 256).requires_grad_(), randn(96, 256, seed=1).requires_grad_(), torch.ones(256, device="cuda")
+    gc.disable()
+    try:
+        for _ in range(2):
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            y, h = rms_norm(x, n, residual=x)
+            z = fp8_linear(h, w)
+            del y, h, z
+            after = torch.cuda.memory_allocated()
+        assert after == before
+    finally:
+        gc.enable()
