@@ -160,8 +160,9 @@ __device__ __forceinline__ void hold(void* p, float* scales, int64_t at, bool li
       const uint32_t r = h[2 * i + q];
       if constexpr (ROOT) {
         // upper half of the noise, four places up; above zero at least the smallest code
+        // (a root above zero over the largest scale is 2^-130 or more)
         const float d = dither(yy[q], (r >> 12) & 0xffff0u);
-        c[2 * i + q] = fmaxf(d, fminf(yy[q] * 1e30f, 0.001953125f));
+        c[2 * i + q] = fmaxf(d, fminf(yy[q] * 0x1p127f, 0.001953125f));
       } else {
         c[2 * i + q] = copysignf(dither(fabsf(yy[q]), lower(r) << 4), yy[q]);
       }
