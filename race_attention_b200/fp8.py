@@ -252,8 +252,10 @@ class Fp8Linear(nn.Module):
 
     The parameter ``weight`` [out_features, in_features] stays in float32 or
     bfloat16 and is quantised on each training pass.  ``hold()`` quantises it
-    once for serving; ``release()`` drops that copy.  A held copy does not
-    follow later changes of ``weight``: training mode ignores it."""
+    once for serving; ``release()`` drops that copy.  Training mode ignores it,
+    and where the weight has changed since (a loaded state, an optimizer's step,
+    another device or type) the next serving call quantises it again.  Writes
+    through ``weight.data`` cannot be seen: call ``hold()`` after them."""
 
     def __init__(self, in_features: int, out_features: int, device=None, dtype=None):
         super().__init__()
@@ -264,13 +266,34 @@ class Fp8Linear(nn.Module):
 
     def hold(self) -> "Fp8Linear":
         self.held = quantize_fp8(self.weight, square=True)
+        self._held_at = self._version()
         return self
 
     def release(self) -> "Fp8Linear":
         self.held = None
         return self
 
+    def _version(self) -> int:
+        """Counts the writes into the weight that torch knows of."""
+        return -1 if self.weight.is_inference() else self.weight._version
+
+    def __setattr__(self, name, value):
+        if name == "weight":
+            self.__dict__["_held_at"] = None       # another tensor, another count
+        super().__setattr__(name, value)
+
+    def __setstate__(self, state):                 # a copy's weight is another tensor too
+        super().__setstate__(state)
+        self._held_at = None
+
+    def _apply(self, fn, recurse=True):            # .to(), .bfloat16(), ...
+        super()._apply(fn, recurse)
+        self._held_at = None
+        return self
+
     def forward(self, x, out_dtype: Optional[torch.dtype] = None):
         if self.held is not None and not self.training:
+            if self._held_at != self._version():
+                self.hold()
             return fp8_linear(x, self.held, out_dtype)
         return fp8_linear(x, self.weight, out_dtype)

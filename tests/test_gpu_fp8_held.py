@@ -1,0 +1,99 @@
+"""A layer's weight held in 8 bits follows the weight (needs a B200)."""
+import copy
+import io
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from race_attention_b200 import _lib
+    _lib.load()
+
+
+def layer(seed):
+    from race_attention_b200.fp8 import Fp8Linear
+    torch.manual_seed(seed)
+    return Fp8Linear(256, 96, device="cuda")
+
+
+def fresh(m, x):
+    """What a layer with this weight, held now, gives."""
+    from race_attention_b200.fp8 import fp8_linear, quantize_fp8
+    return fp8_linear(x, quantize_fp8(m.weight, square=True))
+
+
+def step(m):
+    from race_attention_b200.optim import AdamW
+    m.weight.grad = torch.ones_like(m.weight)
+    AdamW([m.weight], lr=0.1).step()
+    m.weight.grad = None
+
+
+def torch_step(m):
+    m.weight.grad = torch.ones_like(m.weight)
+    torch.optim.SGD([m.weight], lr=0.1).step()
+    m.weight.grad = None
+
+
+def trained(m):
+    m.train()
+    step(m)
+    m.eval()
+
+
+def replaced(m):
+    m.weight = layer(5).weight
+
+
+CHANGES = {"state": lambda m: m.load_state_dict(layer(1).state_dict()),
+           "assigned state": lambda m: m.load_state_dict(layer(1).state_dict(), assign=True),
+           "step": step, "torch's step": torch_step, "training": trained, "type": lambda m: m.bfloat16(),
+           "in place": lambda m: m.weight.detach().mul_(2), "replaced": replaced,
+           "host and back": lambda m: m.cpu().cuda()}
+
+
+@pytest.mark.parametrize("change", CHANGES.values(), ids=CHANGES.keys())
+@torch.no_grad()
+def test_a_held_weight_follows(change):
+    m, x = layer(0).eval().hold(), torch.randn(7, 256, device="cuda")
+    before = m(x)
+    held = m.held
+    assert torch.equal(before, fresh(m, x)) and m(x) is not None and m.held is held     # laid out once
+    change(m)
+    got = m(x)
+    assert torch.equal(got, fresh(m, x)) and m.held is not held
+    again = m.held
+    assert torch.equal(m(x), got) and m.held is again
+    if change not in (CHANGES["host and back"],):
+        assert not torch.equal(got, before)
+
+
+@torch.no_grad()
+def test_a_copy_follows_its_own_weight():
+    m, x = layer(0), torch.randn(7, 256, device="cuda")
+    for _ in range(3):
+        m.weight.mul_(1.5)
+    m.eval().hold()
+    ref = m(x)
+    f = io.BytesIO()
+    torch.save(m, f)
+    f.seek(0)
+    for c in (copy.deepcopy(m), torch.load(f, weights_only=False)):
+        assert torch.equal(c(x), ref)
+        c = copy.deepcopy(m)
+        for _ in range(3):
+            c.weight.mul_(2)
+        assert torch.equal(c(x), fresh(c, x)) and torch.equal(m(x), ref)
+
+
+def test_a_weight_without_a_count():
+    with torch.inference_mode():
+        m, x = layer(0).eval().hold(), torch.randn(7, 256, device="cuda")
+        held = m.held
+        assert torch.equal(m(x), fresh(m, x)) and m.held is held
