@@ -356,6 +356,7 @@ typedef struct {
  * in by_cols, which receives x transposed ([cols][rows]).  square = 1: one
  * scale for each 128 x 128 block; by_cols receives the same codes transposed,
  * and its scales ([column block][row block]) where by_cols.scales is given.
+ * At most 65535 * 128 rows a call: longer ones go in parts of whole blocks.
  * Either output may be left out (codes = NULL), not both.  Bytes between the
  * last column of by_rows (the last row in by_cols) and the next multiple of 16
  * are set to zero. */

@@ -20,6 +20,7 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 constexpr int64_t kBlock = 128;
+constexpr int64_t kRowsAtOnce = 65535 * kBlock;    // of race_quantize
 constexpr auto kF8 = at::kFloat8_e4m3fn;
 
 struct RaceFailure : std::runtime_error {
@@ -87,7 +88,20 @@ std::pair<Held, Held> quantize_rows(const Tensor& x, bool square, int mode) {
   if (square) s = at::empty({blocks_of(r), blocks_of(k)}, x.options().dtype(at::kFloat));
   if (mode != kCols) a = {new_codes(r, k, x), square ? s : new_scales(r, k, x)};
   if (mode != kRows) t = {new_codes(k, r, x), square ? s.t() : new_scales(k, r, x)};
-  check(race_quantize(rr(x), code_of(x), r, k, square, rb(a), rb(t), stream_of(x)));
+  // A launch takes kRowsAtOnce rows, whole blocks, so that longer tensors go in parts.
+  for (int64_t r0 = 0; r0 < r; r0 += kRowsAtOnce) {
+    race_rows_t part{static_cast<char*>(x.data_ptr()) + r0 * x.stride(0) * x.element_size(), x.stride(0)};
+    race_blocks_t by_rows = rb(a), by_cols = rb(t);
+    if (r0 > 0 && mode != kCols) {
+      by_rows.codes = static_cast<char*>(by_rows.codes) + r0 * by_rows.ld;
+      by_rows.scales += (square ? r0 / kBlock : r0) * by_rows.stride_row;
+    }
+    if (r0 > 0 && mode != kRows) {
+      by_cols.codes = static_cast<char*>(by_cols.codes) + r0;
+      by_cols.scales += r0 / kBlock * by_cols.stride_block;
+    }
+    check(race_quantize(part, code_of(x), std::min(r - r0, kRowsAtOnce), k, square, by_rows, by_cols, stream_of(x)));
+  }
   return {a, t};
 }
 
