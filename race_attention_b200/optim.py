@@ -105,6 +105,23 @@ class AdamW(torch.optim.Optimizer):
                 t = torch.cat((b, t.view(b.dtype))).view(dtype if old.dtype == F8 else old.dtype)
             setattr(self, name, t)
 
+    _KEPT = ("state_bits", "seed", "offsets", "_total", "_plans", "exp_avg", "exp_avg_sq", "exp_avg_scale",
+             "exp_avg_sq_scale")
+
+    def __getstate__(self):
+        kept = {name: getattr(self, name) for name in self._KEPT}
+        if self.state_bits == 8:               # as bytes: pickle knows no 8-bit float storage
+            kept.update({n: None if kept[n] is None else kept[n].view(torch.uint8) for n in ("exp_avg", "exp_avg_sq")})
+        return {**super().__getstate__(), **kept}
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        if self.state_bits == 8 and self.exp_avg is not None:
+            self.exp_avg, self.exp_avg_sq = self.exp_avg.view(F8), self.exp_avg_sq.view(F8)
+        for group, (_, _, steps) in zip(self.param_groups, self._plans):
+            for p, s in zip(group["params"], steps):
+                self.state[p]["step"] = s      # views again: a copy of a view is none
+
     def set_state(self, step: int, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor,
                   exp_avg_scale: Optional[torch.Tensor] = None,
                   exp_avg_sq_scale: Optional[torch.Tensor] = None) -> None:
