@@ -142,18 +142,28 @@ class AdamW(torch.optim.Optimizer):
             steps.fill_(int(step))
 
     def state_dict(self):
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
         groups, index = [], {}
         for g in self.param_groups:
             for p in g["params"]:
                 index[p] = len(index)
             groups.append({**{k: v for k, v in g.items() if k != "params"},
                            "params": [index[p] for p in g["params"]]})
-        return {"state": {index[p]: {"step": int(self.state[p]["step"]), "first": self.offsets[p]} for p in index},
-                "param_groups": groups, "state_bits": self.state_bits, "seed": self.seed,
-                "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq,
-                "exp_avg_scale": self.exp_avg_scale, "exp_avg_sq_scale": self.exp_avg_sq_scale}
+        out = {"state": {index[p]: {"step": int(self.state[p]["step"]), "first": self.offsets[p]} for p in index},
+               "param_groups": groups, "state_bits": self.state_bits, "seed": self.seed,
+               "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq,
+               "exp_avg_scale": self.exp_avg_scale, "exp_avg_sq_scale": self.exp_avg_sq_scale}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            other = hook(self, out)
+            out = out if other is None else other
+        return out
 
     def load_state_dict(self, state_dict) -> None:
+        state_dict = dict(state_dict)          # a hook may change it
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            other = hook(self, state_dict)
+            state_dict = state_dict if other is None else other
         if state_dict["state_bits"] != self.state_bits:
             raise ValueError(f"the states were kept in {state_dict['state_bits']} bits, this "
                              f"optimizer has {self.state_bits}")
@@ -173,6 +183,8 @@ class AdamW(torch.optim.Optimizer):
         for g, s in zip(self.param_groups, groups):
             g.update({k: v for k, v in s.items() if k != "params"})
         self.seed = int(state_dict["seed"]) & 0xFFFFFFFF
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     @torch.no_grad()
     def step(self, closure=None):

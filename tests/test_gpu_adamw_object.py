@@ -52,3 +52,21 @@ def test_a_copy_goes_on_by_itself(how, bits):
     twin.add_param_group({"params": [torch.nn.Parameter(torch.ones(5, device="cuda"))]})
     step(twin, 4)
     assert int(twin.state[twin.param_groups[-1]["params"][0]]["step"]) == 1
+
+
+def test_state_dict_hooks_run():
+    from race_attention_b200.optim import AdamW
+    ps = params()
+    opt = AdamW(ps, lr=0.1, state_bits=8)
+    step(opt, 1)
+    seen = []
+    opt.register_state_dict_pre_hook(lambda o: seen.append("before"))
+    opt.register_state_dict_post_hook(lambda o, s: s | {"epoch": 7})
+    opt.register_load_state_dict_pre_hook(lambda o, s: s | {"seed": s["seed"] + 1})
+    opt.register_load_state_dict_post_hook(lambda o: seen.append("after"))
+    saved = opt.state_dict()
+    assert seen == ["before"] and saved["epoch"] == 7 and saved["seed"] == 0
+    step(opt, 2)
+    opt.load_state_dict(saved)
+    assert seen == ["before", "after"] and opt.seed == 1 and saved["seed"] == 0
+    assert [int(opt.state[p]["step"]) for p in ps] == [1, 1, 1]
