@@ -68,7 +68,7 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("parameters must be float32 or bfloat16")
                 if not p.is_contiguous():
                     raise ValueError("parameters must be contiguous")
-                if p.device != self._device(group):
+                if p.device != self._device():
                     raise ValueError("all parameters must be on one device")
         except ValueError:
             self.param_groups.pop()
@@ -84,14 +84,13 @@ class AdamW(torch.optim.Optimizer):
             self.state[p]["step"] = s      # a view: the step counts it up
         self._grow(self._total - before)
 
-    def _device(self, group) -> torch.device:
-        for g in self.param_groups:
-            for p in g["params"]:
-                return p.device
-        return group["params"][0].device
+    def _device(self) -> Optional[torch.device]:
+        return next((p.device for g in self.param_groups for p in g["params"]), None)
 
     def _grow(self, n: int) -> None:
-        dev = self._device(self.param_groups[0])
+        dev = self._device()
+        if dev is None:                        # groups without parameters so far
+            return
         dtype = torch.float32 if self.state_bits == 32 else F8
         new = {"exp_avg": torch.zeros(n, dtype=dtype, device=dev),
                "exp_avg_sq": torch.zeros(n, dtype=dtype, device=dev)}
@@ -174,7 +173,7 @@ class AdamW(torch.optim.Optimizer):
         order = [i for g in groups for i in g["params"]]
         if any(state_dict["state"][i]["first"] != self.offsets[p] for i, p in zip(order, params)):
             raise ValueError("the parameters' sizes differ from this optimizer's")
-        dev = self.exp_avg.device
+        dev = self._device()
         names = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
         self.set_state(0, *(None if state_dict[n] is None else state_dict[n].to(dev, copy=True)
                             for n in names))
@@ -193,6 +192,8 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group, (first, sizes, steps) in zip(self.param_groups, self._plans):
+            if not sizes:
+                continue
             b1, b2 = group["betas"]
             _ops.adamw(group["params"], first, sizes, steps, self.exp_avg, self.exp_avg_sq,
                        self.exp_avg_scale, self.exp_avg_sq_scale, group["lr"], b1, b2, group["eps"],

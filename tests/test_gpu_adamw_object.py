@@ -70,3 +70,19 @@ def test_state_dict_hooks_run():
     opt.load_state_dict(saved)
     assert seen == ["before", "after"] and opt.seed == 1 and saved["seed"] == 0
     assert [int(opt.state[p]["step"]) for p in ps] == [1, 1, 1]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_groups_without_parameters_beside_others(bits):
+    from race_attention_b200.optim import AdamW
+    a, b = params(), params()
+    one = AdamW([{"params": []}, {"params": a, "lr": 0.1}, {"params": []}], state_bits=bits)
+    two = AdamW(b, lr=0.1, state_bits=bits)
+    for s in (1, 2):
+        step(one, s)
+        step(two, s)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    late = AdamW([{"params": []}], state_bits=bits)
+    late.add_param_group({"params": [torch.nn.Parameter(p.detach().clone()) for p in a], "lr": 0.1})
+    step(late, 1)
+    late.load_state_dict(late.state_dict())
