@@ -71,6 +71,10 @@ class BlockFp8:
     def shape(self) -> torch.Size:
         return self.codes.shape
 
+    def _by_square(self) -> bool:
+        """Whether the scales serve as those of square blocks: one row's are both kinds."""
+        return self.square or self.codes.shape[0] <= 1
+
     def dequantize(self) -> torch.Tensor:
         """The values in float32 (for inspection and tests)."""
         s = self.scales.repeat_interleave(BLOCK, 1)[:, :self.codes.shape[1]]
@@ -120,7 +124,7 @@ def fp8_matmul(a: BlockFp8, b: BlockFp8, out_dtype: torch.dtype = torch.bfloat16
     codes = a.codes
     if not codes.is_cuda:
         raise RuntimeError("fp8_matmul runs on CUDA devices only (no CPU fallback)")
-    return _ops.matmul(codes, a.scales, a.square, b.codes, b.scales, b.square, out_dtype == torch.float32,
+    return _ops.matmul(codes, a.scales, a.square and codes.shape[0] > 1, b.codes, b.scales, b.square, out_dtype == torch.float32,
                        out, host_status.word(codes.device))
 
 
@@ -128,7 +132,7 @@ def _check_pair(w: BlockFp8, t: BlockFp8) -> None:
     """t as the transpose of the held weight w: what can be seen without reading the codes."""
     c, d = w.codes, t.codes
     n, k = c.shape
-    if not t.square or d.device != c.device or d.shape != (k, n):
+    if not t._by_square() or d.device != c.device or d.shape != (k, n):
         raise ValueError(f"the transpose that goes with a held weight [{n}, {k}] needs square blocks, "
                          f"[{k}, {n}], on the weight's device")
     if n > 1 and d.data_ptr() == c.data_ptr() and d.stride() == c.stride():
@@ -187,7 +191,7 @@ def fp8_linear(x: Union[torch.Tensor, BlockFp8], weight: Weight,
             raise ValueError("x and weight must be on the same device")
         return _ops.linear(x, weight, None, None, None, None, f32, status)
     w, t = held
-    if not w.square or w.codes.device != x.device:
+    if not w._by_square() or w.codes.device != x.device:
         raise ValueError("a held weight needs square blocks, on x's device")
     if t is None:
         if torch.is_grad_enabled() and x.requires_grad:

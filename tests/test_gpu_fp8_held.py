@@ -97,3 +97,26 @@ def test_a_weight_without_a_count():
         m, x = layer(0).eval().hold(), torch.randn(7, 256, device="cuda")
         held = m.held
         assert torch.equal(m(x), fresh(m, x)) and m.held is held
+
+
+def test_one_row_serves_as_either_kind():
+    """One row has the same scales by rows and by blocks: both are taken wherever one is."""
+    from race_attention_b200.fp8 import BlockFp8, fp8_linear, fp8_matmul, quantize_fp8
+    x, w = torch.randn(1, 300, device="cuda"), torch.randn(1, 300, device="cuda")
+    a, s = quantize_fp8(x), quantize_fp8(x, square=True)
+    h, t = quantize_fp8(w, square=True, transposed=True)
+    again = BlockFp8(h.codes, h.scales)                       # as a program that stored both would
+    ref = fp8_matmul(a, h, torch.float32)
+    for left in (a, s):
+        for right in (h, again, quantize_fp8(w)):
+            assert torch.equal(fp8_matmul(left, right, torch.float32), ref)
+    assert torch.equal(fp8_linear(x, again), ref) and torch.equal(fp8_linear(x, quantize_fp8(w)), ref)
+    z = torch.randn(5, 1, device="cuda").requires_grad_()      # and as the transpose of one column
+    v, u = quantize_fp8(torch.randn(300, 1, device="cuda"), square=True, transposed=True)
+    grads = [torch.autograd.grad(fp8_linear(z, (v, q)), z, torch.ones(5, 300, device="cuda"))[0]
+             for q in (u, BlockFp8(u.codes, u.scales.clone()))]
+    assert grads[0].shape == z.shape and torch.equal(*grads)
+    with pytest.raises(ValueError, match="square"):
+        fp8_linear(x, quantize_fp8(torch.randn(2, 300, device="cuda")))
+    with pytest.raises(ValueError, match="scale for each row"):
+        fp8_matmul(quantize_fp8(torch.randn(2, 300, device="cuda"), square=True), h)
