@@ -46,7 +46,9 @@ int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
 // x as [rows, columns] with contiguous columns; x is float32 or bfloat16
 Tensor rows_of(const Tensor& x) {
-  Tensor r = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  int64_t rows = 1;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
+  Tensor r = x.dim() == 2 ? x : x.reshape({rows, x.size(-1)});
   if ((r.size(1) > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < r.size(1))) r = r.contiguous();
   return r;
 }
