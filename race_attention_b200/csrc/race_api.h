@@ -6,6 +6,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "race_b200.h"
 
 namespace race {
@@ -31,6 +33,19 @@ struct ApiCall {
 // box_rows x 128 bytes with the 128-byte swizzle, zeros outside.
 bool api_encode_bytes(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld,
                       int box_rows);
+
+// Opts a kernel in to its shared memory, once on each device.
+inline int api_allow_smem(const void* fn, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return api_cuda_fail(e);
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (ready.load(std::memory_order_relaxed) & bit) return RACE_OK;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return api_cuda_fail(e);
+  ready.fetch_or(bit, std::memory_order_relaxed);
+  return RACE_OK;
+}
 
 // p lies on a multiple of `bytes` (a null pointer does)
 inline bool api_aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

@@ -407,26 +407,13 @@ __global__ void __launch_bounds__(kSplitThreads)
   }
 }
 
-// Opts a kernel in to its shared memory, once on each device.
-int allow_smem(const void* fn, int bytes, std::atomic<uint64_t>& ready) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return api_cuda_fail(e);
-  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-  if (ready.load(std::memory_order_relaxed) & bit) return RACE_OK;
-  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return api_cuda_fail(e);
-  ready.fetch_or(bit, std::memory_order_relaxed);
-  return RACE_OK;
-}
-
 template <int NT>
 int launch_split(const Args& a, const CUtensorMap& mw, const CUtensorMap& mx, bool square,
                  cudaStream_t s) {
   void (*fn)(CUtensorMap, CUtensorMap, Args) =
       square ? k_mm_split<NT, true> : k_mm_split<NT, false>;
   static std::atomic<uint64_t> ready[2];
-  RACE_CALL(allow_smem(reinterpret_cast<const void*>(fn), Split<NT>::BYTES, ready[square]));
+  RACE_CALL(api_allow_smem(reinterpret_cast<const void*>(fn), Split<NT>::BYTES, ready[square]));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.ranks * ((a.m + NT - 1) / NT)), (unsigned)((a.n + 127) / 128));
   cfg.blockDim = dim3(kSplitThreads);
@@ -905,7 +892,7 @@ template <bool SQ>
 int launch_pair(const PairArgs& p, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& my,
                 cudaStream_t s) {
   static std::atomic<uint64_t> ready;
-  RACE_CALL(allow_smem(reinterpret_cast<const void*>(&k_mm_pair<SQ>), Pair<SQ>::BYTES, ready));
+  RACE_CALL(api_allow_smem(reinterpret_cast<const void*>(&k_mm_pair<SQ>), Pair<SQ>::BYTES, ready));
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
   const int64_t pairs = api_sm_count() / 2;
   cudaLaunchConfig_t cfg{};

@@ -536,27 +536,21 @@ void launch_fwd(const FwdArgs& a, cudaStream_t s) {
   else
     launch_fwd_as<T, VEC, V, WPR, false>(a, s);
 }
-// Returns the CTAs launched: one partial row of dweight each.
+// grid: the CTAs launched, one partial row of dweight each.
 template <typename T, bool VEC, int V, int WPR>
-int launch_bwd(const BwdArgs& a, int most, cudaStream_t s) {
+int launch_bwd(const BwdArgs& a, int most, int& grid, cudaStream_t s) {
   constexpr bool STAGED = VEC && WPR <= 4;
   const int per = STAGED ? Staged<T, V, WPR>::BLOCKS : bwd_blocks(WPR);
-  const int grid = std::min(most, per * api_sm_count());
+  grid = std::min(most, per * api_sm_count());
   if constexpr (STAGED) {
     using L = Staged<T, V, WPR>;
     static std::atomic<uint64_t> ready;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-    if (!(ready.load(std::memory_order_relaxed) & bit)) {
-      cudaFuncSetAttribute(k_rms_bwd_staged<T, V, WPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
-      ready.fetch_or(bit, std::memory_order_relaxed);
-    }
+    RACE_CALL(api_allow_smem(reinterpret_cast<const void*>(&k_rms_bwd_staged<T, V, WPR>), L::BYTES, ready));
     k_rms_bwd_staged<T, V, WPR><<<grid, bwd_threads(WPR), L::BYTES, s>>>(a);
   } else {
     k_rms_bwd<T, VEC, V, WPR><<<grid, bwd_threads(WPR), 0, s>>>(a);
   }
-  return grid;
+  return RACE_OK;
 }
 
 // The spans a warp holds (V) follow from the width; the unvectorised form and
@@ -683,10 +677,11 @@ extern "C" int race_rms_norm_backward(const race_norm_desc_t* desc, race_rows_t 
   const int wpr = norm::warps_per_row(desc->width);
   const int v = (int)((desc->width + 256 * wpr - 1) / (256 * wpr));
   const int most = norm::bwd_ctas(desc, wpr);
-  int grid = 0;
+  int grid = 0, rc = RACE_OK;
   norm::pick(f32, vec, wpr, v, [&](auto t, auto ve, auto vv, auto ww) {
-    grid = norm::launch_bwd<decltype(t), decltype(ve)::value, decltype(vv)::value, decltype(ww)::value>(a, most, stream);
+    rc = norm::launch_bwd<decltype(t), decltype(ve)::value, decltype(vv)::value, decltype(ww)::value>(a, most, grid, stream);
   });
+  RACE_CALL(rc);
   api_log("rms_bwd");
   norm::k_rms_dweight<<<(unsigned)((desc->width + 31) / 32), 1024, 0, stream>>>(
       a.part, grid, a.width, dweight, wb);
