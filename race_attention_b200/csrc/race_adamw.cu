@@ -6,7 +6,7 @@
 //
 // Nothing is used twice, so memory bounds the step: float32 with 32-bit states
 // moves 28 bytes a parameter (96 M parameters 393 us, the copy bandwidth), with 8-bit
-// states 16.1 (266 us, 5.8 TB/s).  bfloat16 with 8-bit states moves 10.1 and is bound by
+// states 16.1 (277 us, 5.6 TB/s).  bfloat16 with 8-bit states moves 10.1 and is bound by
 // its 90 instructions a parameter, half of them logic (184 M: 514 us, 3.6 TB/s).  The tensors'
 // addresses travel in the kernel's parameters (up to 384 tensors in the 32 KB
 // that a launch carries), so a step needs no copy to the device; the step's count,
@@ -285,7 +285,7 @@ struct Ahead {
 // parameters in 97 tensors 677 us, in one tensor 548): bfloat16 parameters go
 // through kRounds times 2048 elements a CTA, the next ones loaded before the current
 // ones are computed (514 us).  float32 moves 16 bytes a parameter, memory is the
-// bound again, and one round with more CTAs is faster (96 M: 266 us against 299).
+// bound again, and one round with more CTAs is faster (by 11 % at 100.7 M).
 template <int N, bool HALF>
 __device__ __forceinline__ void steps8(const Args<N>& a, const Item& it, int64_t c0) {
   using T = typename std::conditional<HALF, bf16, float>::type;
@@ -356,9 +356,11 @@ __device__ __forceinline__ void steps8(const Args<N>& a, const Item& it, int64_t
   }
 }
 
-// one type of parameters a launch: the two forms need 48 and 66 registers
+// One type of parameters a launch: the two forms need 48 and 67 registers.  The
+// compiler would take 50 for float32, which leaves four CTAs an SM in place of five
+// (96.0 M parameters 295 us in place of 277).
 template <int N, bool HALF>
-__global__ void __launch_bounds__(NT) k_adamw8(const __grid_constant__ Args<N> a) {
+__global__ void __launch_bounds__(NT, HALF ? 3 : 5) k_adamw8(const __grid_constant__ Args<N> a) {
   const int chunk = blockIdx.x, lo = tensor_of(a, chunk);
   const int64_t c0 = (int64_t)(chunk - (lo > 0 ? a.end[lo - 1] : 0)) * kChunk;
   steps8<N, HALF>(a, a.item[lo], c0 * (HALF ? kRounds : 1));
