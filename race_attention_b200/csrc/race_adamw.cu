@@ -5,10 +5,12 @@
 //   p -= lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Nothing is used twice, so memory bounds the step: float32 with 32-bit states
-// moves 28 bytes a parameter (96 M parameters 393 us, the copy bandwidth), with 8-bit
-// states 16.1 (277 us, 5.6 TB/s).  bfloat16 with 8-bit states moves 10.1 and is bound by
-// its 90 instructions a parameter, half of them logic (184 M: 514 us, 3.6 TB/s).  The tensors'
-// addresses travel in the kernel's parameters (up to 384 tensors in the 32 KB
+// moves 28 bytes a parameter (96.0 M parameters 395 us, 6.8 TB/s; a copy, which writes as
+// much as it reads where the step writes 12 bytes of 28, reaches 6.4), with 8-bit
+// states 16.1 (258 us, 6.0 TB/s; 277 where other work had filled the cache), bfloat16 with
+// 32-bit states 22 (337 us, 6.3).  bfloat16 with 8-bit states moves 10.1 and is bound by
+// its 90 instructions a parameter, half of them logic (184 M: 509 us, 3.7 TB/s).  The tensors'
+// addresses travel in the kernel's parameters (up to 360 tensors in the 32 KB
 // that a launch carries), so a step needs no copy to the device; the step's count,
 // learning rate and noise travel with them, which is why a capture is refused: each
 // replay would repeat them.  A CTA finds its 2048 elements by bisection over the running chunk
@@ -25,6 +27,9 @@
 // bfloat16 parameters (2^-9 of themselves apart) are rounded the same way.
 // The noise is a hash of the element's index, the seed and t, two odd
 // multipliers (2^32 over the golden ratio; the fraction of sqrt(2)) between shifts.
+// m takes its lower half, the root its upper half, and the parameter the lower half
+// under the next key, which for an even key is that of m's neighbour: each rounding
+// is right on average, but the two are not independent.
 #include <cmath>
 #include <type_traits>
 
