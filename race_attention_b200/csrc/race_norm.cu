@@ -391,11 +391,22 @@ __global__ void __launch_bounds__(bwd_threads(WPR), Staged<T, V, WPR>::BLOCKS) k
   }
 }
 
-// CTAs of the form without vector loads that an SM holds
-constexpr int bwd_blocks(int wpr) { return wpr == 1 ? 2 : wpr == 4 ? 4 : 1; }
+// CTAs of the unstaged form that an SM holds
+constexpr int bwd_blocks(int wpr, int v) { return wpr == 1 ? v == 1 ? 3 : 2 : wpr == 4 ? 4 : 1; }
+
+// Where rows wait in shared memory.  A bfloat16 row is short, and several of them have to
+// be on their way; a float32 row of more than 96 columns is on its way in enough
+// registers by itself, and its second reading from shared memory costs more than the
+// wait.  67 M elements with dh, staged against not: float32 1046872 x 64 373 and 403 us,
+// 523432 x 128 283 and 241, 261712 x 256 267 and 175, 65424 x 1024 294 and 179, 16352 x 4096
+// 309 and 191; bfloat16 10904 x 6144 157 and 192, 8176 x 8192 133 and 161, 4088 x 16384
+// 142 and 152 (without dh 8178 x 8192 123 and 116).
+template <typename T, bool VEC, int V, int WPR>
+constexpr bool can_stage() { return VEC && (sizeof(T) == 2 ? WPR <= 16 : V == 1 && WPR == 1); }
+constexpr int kStagedFloats = 96;
 
 template <typename T, bool VEC, int V, int WPR>
-__global__ void __launch_bounds__(bwd_threads(WPR), bwd_blocks(WPR)) k_rms_bwd(const BwdArgs a) {
+__global__ void __launch_bounds__(bwd_threads(WPR), bwd_blocks(WPR, V)) k_rms_bwd(const BwdArgs a) {
   __shared__ float slot[2][32];
   constexpr int RPC = bwd_threads(WPR) / (32 * WPR);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -539,15 +550,18 @@ void launch_fwd(const FwdArgs& a, cudaStream_t s) {
 // grid: the CTAs launched, one partial row of dweight each.
 template <typename T, bool VEC, int V, int WPR>
 int launch_bwd(const BwdArgs& a, int most, int& grid, cudaStream_t s) {
-  constexpr bool STAGED = VEC && WPR <= 4;
-  const int per = STAGED ? Staged<T, V, WPR>::BLOCKS : bwd_blocks(WPR);
-  grid = std::min(most, per * api_sm_count());
-  if constexpr (STAGED) {
-    using L = Staged<T, V, WPR>;
-    static std::atomic<uint64_t> ready;
-    RACE_CALL(api_allow_smem(reinterpret_cast<const void*>(&k_rms_bwd_staged<T, V, WPR>), L::BYTES, ready));
-    k_rms_bwd_staged<T, V, WPR><<<grid, bwd_threads(WPR), L::BYTES, s>>>(a);
-  } else {
+  if constexpr (can_stage<T, VEC, V, WPR>()) {
+    if (sizeof(T) == 2 || a.width <= kStagedFloats) {
+      using L = Staged<T, V, WPR>;
+      static std::atomic<uint64_t> ready;
+      RACE_CALL(api_allow_smem(reinterpret_cast<const void*>(&k_rms_bwd_staged<T, V, WPR>), L::BYTES, ready));
+      grid = std::min(most, L::BLOCKS * api_sm_count());
+      k_rms_bwd_staged<T, V, WPR><<<grid, bwd_threads(WPR), L::BYTES, s>>>(a);
+      return RACE_OK;
+    }
+  }
+  if constexpr (sizeof(T) == 4 || !can_stage<T, VEC, V, WPR>()) {
+    grid = std::min(most, bwd_blocks(WPR, V) * api_sm_count());
     k_rms_bwd<T, VEC, V, WPR><<<grid, bwd_threads(WPR), 0, s>>>(a);
   }
   return RACE_OK;
