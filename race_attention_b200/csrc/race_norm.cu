@@ -14,13 +14,16 @@
 // otherwise (odd widths or strides) lane l holds columns l, l + 32, ... and the
 // whole warp holds a block in four of its eight values.
 //
-// Rows are short (1.5 KB at 768 bfloat16 columns), so a warp that loads one, waits,
+// bfloat16 rows are short (1.5 KB at 768 columns), so a warp that loads one, waits,
 // sums and stores keeps too few bytes on their way.  The grid is what the SMs
 // hold at once and a warp walks rows; with vector loads the next rows are on their way
 // before the current one is summed, in registers (forward, one row) or shared
 // memory (backward, one or two).  Measured, bfloat16 with residual: 65536 x 768 forward
 // 71 us (5.6 TB/s), to 8 bits 61 us (5.8), backward with dweight 82 us (4.9); one row a
-// warp and no row ahead took 79, 83 and 112 to 158.
+// warp and no row ahead took 79, 83 and 112 to 158.  float32 rows are on their way in
+// enough registers by themselves; which form takes which rows stands beside the launches,
+// with both sides measured (float32 with residual: 65104 x 768 forward 124 us, 6.5 TB/s,
+// to 8 bits 101 us, 6.4; 87232 x 768 backward 180 us, 5.9).
 #include <algorithm>
 #include <atomic>
 
@@ -147,11 +150,12 @@ __device__ __forceinline__ float row_sum(float a, float (*slot)[32], int which) 
 
 constexpr int threads_of(int wpr) { return wpr == 1 ? 128 : 32 * wpr; }
 
-template <typename T, bool VEC, int V, int WPR, bool Q>
-__global__ void __launch_bounds__(threads_of(WPR)) k_rms_fwd(const FwdArgs a) {
+// WALK: whether a row's warps go on to further rows.
+template <typename T, bool VEC, int V, int WPR, bool Q, bool WALK>
+__global__ void __launch_bounds__(threads_of(WPR), WPR == 32 && !VEC && Q ? 1 : 0) k_rms_fwd(const FwdArgs a) {
   __shared__ float slot[2][32];
   constexpr int RPC = threads_of(WPR) / (32 * WPR);
-  constexpr bool AHEAD = VEC && V * sizeof(T) <= 8;         // the next row waits in registers
+  constexpr bool AHEAD = WALK && VEC && V * sizeof(T) <= 8;   // the next row waits in registers
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int w0 = warp % WPR;
   const int64_t step = (int64_t)gridDim.x * RPC;
@@ -164,7 +168,7 @@ __global__ void __launch_bounds__(threads_of(WPR)) k_rms_fwd(const FwdArgs a) {
     if (res != nullptr) nr.load(res + row * a.ldr, w0, WPR, lane, a.width);
   }
   int which = 0;
-  for (; row < a.rows; row += step) {
+  for (; row < a.rows; row = WALK ? row + step : a.rows) {
     float h[V][8];
     if constexpr (AHEAD) {
 #pragma unroll
@@ -185,12 +189,17 @@ __global__ void __launch_bounds__(threads_of(WPR)) k_rms_fwd(const FwdArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) load_span<T, VEC>(x + row * a.ldx, j * WPR + w0, lane, a.width, h[j]);
       if (res != nullptr) {
+        // single elements of one row: all of the residual's on their way before the first is added
+        constexpr int G = WALK || VEC || WPR == 32 ? 1 : V;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float t[8];
-          load_span<T, VEC>(res + row * a.ldr, j * WPR + w0, lane, a.width, t);
+        for (int j0 = 0; j0 < V; j0 += G) {
+          float t[G][8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h[j][i] += t[i];
+          for (int j = 0; j < G; ++j) load_span<T, VEC>(res + row * a.ldr, (j0 + j) * WPR + w0, lane, a.width, t[j]);
+#pragma unroll
+          for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[j0 + j][i] += t[j][i];
         }
       }
     }
@@ -532,20 +541,49 @@ int64_t resident(K kernel, int threads, std::atomic<int>& held) {
   return (int64_t)n * api_sm_count();
 }
 
-template <typename T, bool VEC, int V, int WPR, bool Q>
+template <typename T, bool VEC, int V, int WPR, bool Q, bool WALK>
 void launch_fwd_as(const FwdArgs& a, cudaStream_t s) {
   constexpr int RPC = threads_of(WPR) / (32 * WPR);
-  static std::atomic<int> held;
-  const int64_t most = (a.rows + RPC - 1) / RPC;
-  const int64_t fill = resident(&k_rms_fwd<T, VEC, V, WPR, Q>, threads_of(WPR), held);
-  k_rms_fwd<T, VEC, V, WPR, Q><<<(unsigned)(most < fill ? most : fill), threads_of(WPR), 0, s>>>(a);
+  int64_t grid = (a.rows + RPC - 1) / RPC;
+  if constexpr (WALK) {
+    static std::atomic<int> held;
+    grid = std::min(grid, resident(&k_rms_fwd<T, VEC, V, WPR, Q, true>, threads_of(WPR), held));
+  }
+  k_rms_fwd<T, VEC, V, WPR, Q, WALK><<<(unsigned)grid, threads_of(WPR), 0, s>>>(a);
+}
+
+// Rows walked, or a CTA's rows alone.  Walking pays where a row leaves too few bytes on
+// their way: bfloat16, and narrow float32.  Otherwise the CTAs that come and go keep
+// more of them, and the registers that the loop takes cost more than it saves; a loop
+// over 64 values a thread spills.  50 M elements with residual, walked and not, to x's
+// type and (after the stroke) to 8 bits, in us:
+//   float32           781250 x 64 160, 170 / 193, 204    390625 x 128 127, 120 / 114, 119
+//                     195312 x 256 150, 122 / 118, 98    48828 x 1024 149, 128 / 110, 102
+//                     12207 x 4096 147, 128 / 112, 109   1525 x 32768 555, 237 / 596, 222
+//   bfloat16          1525 x 32768 341, 128 / 322, 133
+//   float32, single   196078 x 255 144, 174 / 148, 183   97847 x 511 134, 124 / 132, 134
+//   elements          49950 x 1001 138, 122 / 133, 125 (without residual 71, 65 / 65, 93)
+//                     9994 x 5003 223, 138 / 249, 170    3050 x 16390 1153, 328 / 333, 507
+//   bfloat16, single  49950 x 1001 93, 91 / 112, 123     31230 x 1601 148, 147 / 199, 183
+//   elements          9994 x 5003 233, 240 / 255, 273    3050 x 16390 1040, 281 / 354, 433
+template <typename T, bool VEC, int V, int WPR, bool Q>
+void launch_fwd_by(const FwdArgs& a, cudaStream_t s) {
+  if constexpr (sizeof(T) == 4 && WPR == 1 && (V == 1 || !VEC)) {
+    if (a.width < (VEC ? (Q ? 160 : 96) : (Q ? 1025 : 384)))
+      launch_fwd_as<T, VEC, V, WPR, Q, true>(a, s);
+    else
+      launch_fwd_as<T, VEC, V, WPR, Q, false>(a, s);
+  } else {
+    constexpr bool WALK = WPR == 32 ? !VEC && Q : sizeof(T) == 2 && (VEC || WPR != 4);
+    launch_fwd_as<T, VEC, V, WPR, Q, WALK>(a, s);
+  }
 }
 template <typename T, bool VEC, int V, int WPR>
 void launch_fwd(const FwdArgs& a, cudaStream_t s) {
   if (a.codes != nullptr)
-    launch_fwd_as<T, VEC, V, WPR, true>(a, s);
+    launch_fwd_by<T, VEC, V, WPR, true>(a, s);
   else
-    launch_fwd_as<T, VEC, V, WPR, false>(a, s);
+    launch_fwd_by<T, VEC, V, WPR, false>(a, s);
 }
 // grid: the CTAs launched, one partial row of dweight each.
 template <typename T, bool VEC, int V, int WPR>
