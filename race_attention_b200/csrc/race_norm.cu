@@ -60,21 +60,29 @@ struct BwdArgs {
 };
 
 // column of value i of span s
-template <bool VEC>
+template <int VEC>
 __device__ __forceinline__ int col_of(int s, int lane, int i) {
   return 256 * s + (VEC ? 8 * lane + i : 32 * i + lane);
 }
 
-// Vector loads need every row's base on 16 bytes and whole vectors (width % 8 == 0).
-template <typename T, bool VEC>
+// VEC 0: single elements.  1: vectors, which need every row's base on 16 bytes and
+// width % 8 == 0.  2: the same with width % 8 == 4, float32 alone (and a weight of that
+// type): the last lane that holds columns holds four.
+template <typename T, int VEC>
 __device__ __forceinline__ void load_span(const T* row, int s, int lane, int width, float (&v)[8]) {
   if constexpr (VEC) {
     const int c = 256 * s + 8 * lane;
-    if (c < width) {
+    if (VEC == 1 ? c < width : c + 8 <= width) {
       load8(row + c, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      if constexpr (VEC == 2 && sizeof(T) == 4) {
+        if (c < width) {
+          const float4 f = *reinterpret_cast<const float4*>(row + c);
+          v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        }
+      }
     }
   } else {
 #pragma unroll
@@ -84,11 +92,15 @@ __device__ __forceinline__ void load_span(const T* row, int s, int lane, int wid
     }
   }
 }
-template <typename T, bool VEC>
+template <typename T, int VEC>
 __device__ __forceinline__ void store_span(T* row, int s, int lane, int width, const float (&v)[8]) {
   if constexpr (VEC) {
     const int c = 256 * s + 8 * lane;
-    if (c < width) store8(row + c, v);
+    if (VEC == 1 ? c < width : c + 8 <= width) {
+      store8(row + c, v);
+    } else if constexpr (VEC == 2 && sizeof(T) == 4) {
+      if (c < width) *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -99,7 +111,7 @@ __device__ __forceinline__ void store_span(T* row, int s, int lane, int width, c
 }
 
 // A warp's spans of a row as they were loaded: 4 (bfloat16) or 8 registers a span.
-template <typename T, int V>
+template <typename T, int V, int VEC>
 struct Raw {
   uint4 u[V][sizeof(T) / 2];
   __device__ __forceinline__ void load(const T* row, int w0, int wpr, int lane, int width) {
@@ -108,7 +120,7 @@ struct Raw {
       const int c = 256 * (j * wpr + w0) + 8 * lane;
 #pragma unroll
       for (int q = 0; q < (int)sizeof(T) / 2; ++q)
-        u[j][q] = c < width ? *reinterpret_cast<const uint4*>(row + c + q * (16 / (int)sizeof(T)))
+        u[j][q] = (VEC == 1 ? c : c + 4 * q) < width ? *reinterpret_cast<const uint4*>(row + c + q * (16 / (int)sizeof(T)))
                             : make_uint4(0, 0, 0, 0);
     }
   }
@@ -117,7 +129,7 @@ struct Raw {
   }
 };
 
-template <bool VEC>
+template <int VEC>
 __device__ __forceinline__ void load_weight(const void* w, int wbf16, int s, int lane, int width,
                                             float (&v)[8]) {
   if (wbf16)
@@ -151,7 +163,7 @@ __device__ __forceinline__ float row_sum(float a, float (*slot)[32], int which) 
 constexpr int threads_of(int wpr) { return wpr == 1 ? 128 : 32 * wpr; }
 
 // WALK: whether a row's warps go on to further rows.
-template <typename T, bool VEC, int V, int WPR, bool Q, bool WALK>
+template <typename T, int VEC, int V, int WPR, bool Q, bool WALK>
 __global__ void __launch_bounds__(threads_of(WPR), WPR == 32 && !VEC && Q ? 1 : 0) k_rms_fwd(const FwdArgs a) {
   __shared__ float slot[2][32];
   constexpr int RPC = threads_of(WPR) / (32 * WPR);
@@ -162,7 +174,7 @@ __global__ void __launch_bounds__(threads_of(WPR), WPR == 32 && !VEC && Q ? 1 : 
   int64_t row = (int64_t)blockIdx.x * RPC + warp / WPR;     // the same for a row's warps
   const T* x = static_cast<const T*>(a.x);
   const T* res = static_cast<const T*>(a.res);
-  Raw<T, V> nx, nr;
+  Raw<T, V, VEC> nx, nr;
   if (AHEAD && row < a.rows) {
     nx.load(x + row * a.ldx, w0, WPR, lane, a.width);
     if (res != nullptr) nr.load(res + row * a.ldr, w0, WPR, lane, a.width);
@@ -251,7 +263,7 @@ __global__ void __launch_bounds__(threads_of(WPR), WPR == 32 && !VEC && Q ? 1 : 
             const float inv = 1.f / sv;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int cc = col_of<false>(s, lane, 4 * b + i);
+              const int cc = col_of<0>(s, lane, 4 * b + i);
               // the row's pitch is a multiple of 16: the rest of its last 16 bytes is zeroed
               if (cc < ((a.width + 15) & ~15))
                 c[cc] = (uint8_t)code2(h[j][4 * b + i] * inv, 0.f);
@@ -341,7 +353,7 @@ __global__ void __launch_bounds__(bwd_threads(WPR), Staged<T, V, WPR>::BLOCKS) k
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float w[8], g[8], h[8];
-      load_weight<true>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
+      load_weight<1>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
       get(stage, 0, j, g);
       get(stage, 1, j, h);
 #pragma unroll
@@ -357,7 +369,7 @@ __global__ void __launch_bounds__(bwd_threads(WPR), Staged<T, V, WPR>::BLOCKS) k
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float w[8], g[8], h[8];
-      load_weight<true>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
+      load_weight<1>(a.w, a.wbf16, j * WPR + w0, lane, a.width, w);
       get(stage, 0, j, g);
       get(stage, 1, j, h);
 #pragma unroll
@@ -367,7 +379,7 @@ __global__ void __launch_bounds__(bwd_threads(WPR), Staged<T, V, WPR>::BLOCKS) k
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] += h[i];
       }
-      store_span<T, true>(dx, j * WPR + w0, lane, a.width, g);
+      store_span<T, 1>(dx, j * WPR + w0, lane, a.width, g);
     }
     stage = stage == L::STAGES - 1 ? 0 : stage + 1;
   }
@@ -377,7 +389,7 @@ __global__ void __launch_bounds__(bwd_threads(WPR), Staged<T, V, WPR>::BLOCKS) k
     for (int j = 0; j < V; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int c = col_of<true>(j * WPR + w0, lane, i);
+        const int c = col_of<1>(j * WPR + w0, lane, i);
         if (c < a.width) part[c] = dw[j][i];
       }
   } else {
@@ -388,7 +400,7 @@ __global__ void __launch_bounds__(bwd_threads(WPR), Staged<T, V, WPR>::BLOCKS) k
     for (int j = 0; j < V; ++j) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) red[warp][col_of<true>(0, lane, i)] = dw[j][i];
+      for (int i = 0; i < 8; ++i) red[warp][col_of<1>(0, lane, i)] = dw[j][i];
       __syncthreads();
       for (int c = threadIdx.x; c < 256; c += 32 * RPC) {
         float t = 0.f;
@@ -410,11 +422,11 @@ constexpr int bwd_blocks(int wpr, int v) { return wpr == 1 ? v == 1 ? 3 : 2 : wp
 // 523432 x 128 283 and 241, 261712 x 256 267 and 175, 65424 x 1024 294 and 179, 16352 x 4096
 // 309 and 191; bfloat16 10904 x 6144 157 and 192, 8176 x 8192 133 and 161, 4088 x 16384
 // 142 and 152 (without dh 8178 x 8192 123 and 116).
-template <typename T, bool VEC, int V, int WPR>
-constexpr bool can_stage() { return VEC && (sizeof(T) == 2 ? WPR <= 16 : V == 1 && WPR == 1); }
+template <typename T, int VEC, int V, int WPR>
+constexpr bool can_stage() { return VEC == 1 && (sizeof(T) == 2 ? WPR <= 16 : V == 1 && WPR == 1); }
 constexpr int kStagedFloats = 96;
 
-template <typename T, bool VEC, int V, int WPR>
+template <typename T, int VEC, int V, int WPR>
 __global__ void __launch_bounds__(bwd_threads(WPR), bwd_blocks(WPR, V)) k_rms_bwd(const BwdArgs a) {
   __shared__ float slot[2][32];
   constexpr int RPC = bwd_threads(WPR) / (32 * WPR);
@@ -541,7 +553,7 @@ int64_t resident(K kernel, int threads, std::atomic<int>& held) {
   return (int64_t)n * api_sm_count();
 }
 
-template <typename T, bool VEC, int V, int WPR, bool Q, bool WALK>
+template <typename T, int VEC, int V, int WPR, bool Q, bool WALK>
 void launch_fwd_as(const FwdArgs& a, cudaStream_t s) {
   constexpr int RPC = threads_of(WPR) / (32 * WPR);
   int64_t grid = (a.rows + RPC - 1) / RPC;
@@ -566,7 +578,7 @@ void launch_fwd_as(const FwdArgs& a, cudaStream_t s) {
 //                     9994 x 5003 223, 138 / 249, 170    3050 x 16390 1153, 328 / 333, 507
 //   bfloat16, single  49950 x 1001 93, 91 / 112, 123     31230 x 1601 148, 147 / 199, 183
 //   elements          9994 x 5003 233, 240 / 255, 273    3050 x 16390 1040, 281 / 354, 433
-template <typename T, bool VEC, int V, int WPR, bool Q>
+template <typename T, int VEC, int V, int WPR, bool Q>
 void launch_fwd_by(const FwdArgs& a, cudaStream_t s) {
   if constexpr (sizeof(T) == 4 && WPR == 1 && (V == 1 || !VEC)) {
     if (a.width < (VEC ? (Q ? 160 : 96) : (Q ? 1025 : 384)))
@@ -578,7 +590,7 @@ void launch_fwd_by(const FwdArgs& a, cudaStream_t s) {
     launch_fwd_as<T, VEC, V, WPR, Q, WALK>(a, s);
   }
 }
-template <typename T, bool VEC, int V, int WPR>
+template <typename T, int VEC, int V, int WPR>
 void launch_fwd(const FwdArgs& a, cudaStream_t s) {
   if (a.codes != nullptr)
     launch_fwd_by<T, VEC, V, WPR, true>(a, s);
@@ -586,7 +598,7 @@ void launch_fwd(const FwdArgs& a, cudaStream_t s) {
     launch_fwd_by<T, VEC, V, WPR, false>(a, s);
 }
 // grid: the CTAs launched, one partial row of dweight each.
-template <typename T, bool VEC, int V, int WPR>
+template <typename T, int VEC, int V, int WPR>
 int launch_bwd(const BwdArgs& a, int most, int& grid, cudaStream_t s) {
   if constexpr (can_stage<T, VEC, V, WPR>()) {
     if (sizeof(T) == 2 || a.width <= kStagedFloats) {
@@ -605,23 +617,32 @@ int launch_bwd(const BwdArgs& a, int most, int& grid, cudaStream_t s) {
   return RACE_OK;
 }
 
-// The spans a warp holds (V) follow from the width; the unvectorised form and
+// The spans a warp holds (V) follow from the width; the form of single elements and
 // the widest rows are built once.
 template <typename F>
-void pick(bool f32, bool vec, int wpr, int v, F&& f) {
+void pick(bool f32, int vec, int wpr, int v, F&& f) {
+#define RACE_AS(T, VEC, V, W) \
+  f(T(), std::integral_constant<int, VEC>(), std::integral_constant<int, V>(), std::integral_constant<int, W>())
 #define RACE_PICK(V, W)                                                     \
-  if (wpr == W && (vec || V == (W == 32 ? 8 : 4)) && v <= V) {              \
-    if (vec) return f32 ? f(float(), std::true_type(), std::integral_constant<int, V>(), std::integral_constant<int, W>())  \
-                        : f(bf16(), std::true_type(), std::integral_constant<int, V>(), std::integral_constant<int, W>());  \
+  if (wpr == W && (vec != 0 || V == (W == 32 ? 8 : 4)) && v <= V) {         \
+    if (vec == 2) return RACE_AS(float, 2, V, W);                           \
+    if (vec == 1) return f32 ? RACE_AS(float, 1, V, W) : RACE_AS(bf16, 1, V, W); \
     if constexpr (V == (W == 32 ? 8 : 4))                                   \
-      return f32 ? f(float(), std::false_type(), std::integral_constant<int, V>(), std::integral_constant<int, W>())        \
-                 : f(bf16(), std::false_type(), std::integral_constant<int, V>(), std::integral_constant<int, W>());        \
+      return f32 ? RACE_AS(float, 0, V, W) : RACE_AS(bf16, 0, V, W);        \
   }
   RACE_PICK(1, 1) RACE_PICK(2, 1) RACE_PICK(3, 1) RACE_PICK(4, 1)
   RACE_PICK(2, 4) RACE_PICK(3, 4) RACE_PICK(4, 4)
   RACE_PICK(2, 16) RACE_PICK(3, 16) RACE_PICK(4, 16)
   RACE_PICK(8, 32)
 #undef RACE_PICK
+#undef RACE_AS
+}
+
+// The form of the loads (see load_span) for rows whose bases allow vectors.
+int vec_of(const race_norm_desc_t* d, bool aligned) {
+  if (!aligned) return 0;
+  if (d->width % 8 == 0) return 1;
+  return d->width % 4 == 0 && d->dtype == RACE_F32 && d->weight_dtype == RACE_F32 ? 2 : 0;
 }
 
 bool aligned16(const void* p, int64_t ld, int es) {
@@ -676,13 +697,13 @@ extern "C" int race_rms_norm(const race_norm_desc_t* desc, race_rows_t x, race_r
                   y8.stride_row, y8.stride_block, rstd, desc->rows, (int)desc->width, desc->eps};
   const bool f32 = desc->dtype == RACE_F32;
   const int es = f32 ? 4 : 2;
-  const bool vec = desc->width % 8 == 0 && norm::aligned16(x.data, x.ld, es) && norm::aligned16(weight, 0, 1) &&
+  const bool aligned = norm::aligned16(x.data, x.ld, es) && norm::aligned16(weight, 0, 1) &&
                    (residual.data == nullptr || (norm::aligned16(residual.data, residual.ld, es) &&
                                                  norm::aligned16(h.data, h.ld, es))) &&
                    (y.data == nullptr || norm::aligned16(y.data, y.ld, es));
   const int wpr = norm::warps_per_row(desc->width);
   const int v = (int)((desc->width + 256 * wpr - 1) / (256 * wpr));
-  norm::pick(f32, vec, wpr, v, [&](auto t, auto ve, auto vv, auto ww) {
+  norm::pick(f32, norm::vec_of(desc, aligned), wpr, v, [&](auto t, auto ve, auto vv, auto ww) {
     norm::launch_fwd<decltype(t), decltype(ve)::value, decltype(vv)::value, decltype(ww)::value>(a, stream);
   });
   api_log(y8.codes != nullptr ? "rms_fwd_8bit" : "rms_fwd");
@@ -723,14 +744,14 @@ extern "C" int race_rms_norm_backward(const race_norm_desc_t* desc, race_rows_t 
                   static_cast<float*>(workspace), desc->rows, (int)desc->width};
   const bool f32 = desc->dtype == RACE_F32;
   const int es = f32 ? 4 : 2;
-  const bool vec = desc->width % 8 == 0 && norm::aligned16(dy.data, dy.ld, es) && norm::aligned16(h.data, h.ld, es) &&
+  const bool aligned = norm::aligned16(dy.data, dy.ld, es) && norm::aligned16(h.data, h.ld, es) &&
                    norm::aligned16(dx.data, dx.ld, es) && norm::aligned16(weight, 0, 1) &&
                    (dh.data == nullptr || norm::aligned16(dh.data, dh.ld, es));
   const int wpr = norm::warps_per_row(desc->width);
   const int v = (int)((desc->width + 256 * wpr - 1) / (256 * wpr));
   const int most = norm::bwd_ctas(desc, wpr);
   int grid = 0, rc = RACE_OK;
-  norm::pick(f32, vec, wpr, v, [&](auto t, auto ve, auto vv, auto ww) {
+  norm::pick(f32, norm::vec_of(desc, aligned), wpr, v, [&](auto t, auto ve, auto vv, auto ww) {
     rc = norm::launch_bwd<decltype(t), decltype(ve)::value, decltype(vv)::value, decltype(ww)::value>(a, most, grid, stream);
   });
   RACE_CALL(rc);
