@@ -221,9 +221,10 @@ __global__ void __launch_bounds__(kSplitThreads)
   uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::MISC);
   volatile uint32_t* abort = misc + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int C = a.ranks, tile = (int)blockIdx.x / C, rank = (int)blockIdx.x - tile * C;
+  // ranks are a power of two; divisions by them would stand before the first load
+  const int C = a.ranks, lc = __popc(C - 1), tile = (int)blockIdx.x >> lc, rank = (int)blockIdx.x & (C - 1);
   const int64_t n0 = (int64_t)blockIdx.y * 128, m0 = (int64_t)tile * NT;
-  const int k0 = (int)((int64_t)a.kb * rank / C), k1 = (int)((int64_t)a.kb * (rank + 1) / C);
+  const int k0 = (int)((int64_t)a.kb * rank >> lc), k1 = (int)((int64_t)a.kb * (rank + 1) >> lc);
   const int blocks = k1 - k0;
 
   if (tid == 0) {
