@@ -921,14 +921,17 @@ int launch_pair(const PairArgs& p, const CUtensorMap& ma, const CUtensorMap& mb,
 
 // How a product is cut: the cheaper of the two kernels by their measured times
 // (148 SMs, operands in L2; kb = blocks of the contraction).
-//   k_mm_split: 4 us and 0.39 us a block while every tile has an SM; from about 288
-//     tiles of 64 tokens on, 330 tile-blocks a us (1024 x 2304 x 768 8.1 us, 2048 14.0).
-//     Joining a cluster's ranks costs 1.6 us for 64 tokens and 0.4 us for 16 (and
-//     an SM for each rank: at two ranks an SM 256 x 2304 x 768 takes 11.0 us in place
-//     of 6.3), each rank taken off saves its blocks: 64 x 4096 x 4096 16.5, 12.0,
-//     8.6, 9.8 us for 1, 2, 4, 8 ranks, 16 x 8192 x 8192 25.8, 15.5, 11.7, 16.0.
+//   k_mm_split: 4 us and 0.39 us a block while every CTA has an SM; beyond that 330
+//     tile-blocks a us, a tile's start and end as long as 2.5 of its blocks
+//     (1024 x 2304 x 768 7.8 us, 2048 x 1536 x 768 12.2, 16384 x 384 x 384 14.5).  Joining a
+//     cluster's ranks costs 1.6 us for 64 tokens and 0.4 us for 16, eight ranks 0.4 more;
+//     each rank taken off saves its blocks (33 x 768 x 3000 7.0 us for 4 ranks, 6.0 for 8;
+//     16 x 8192 x 8192 25.8, 15.5, 11.7, 16.0 for 1, 2, 4, 8).  Two of a cluster's ranks on one SM
+//     start 1.7 us later and take 0.48 us a block, eight of them join in 1.6 us more:
+//     that pays where a rank keeps many blocks (128 x 8192 x 8192 22.4 us against 29.5 without,
+//     256 x 4096 x 4096 14.5 and 16.7, 256 x 2304 x 768 11.0 and 6.3).
 //   k_mm_pair: 6.4 us, and 0.45 us a block and 1 us a tile for every round of the 74
-//     pairs (2048 x 2304 x 768 9.2 us, 1024 x 4096 x 4096 20.2); a contraction cut in
+//     pairs (2048 x 1536 x 768 8.9 us, 1024 x 4096 x 4096 20.2); a contraction cut in
 //     s adds 2.5 us and the partial results' way at 5 TB/s.
 struct Plan {
   bool pair;
@@ -942,12 +945,13 @@ Plan plan_of(int64_t m, int64_t n, int64_t k) {
   p.nt = m <= 16 ? 16 : m <= 32 ? 32 : 64;
   const double join = p.nt == 64 ? 1.6 : 0.4;
   const int64_t tiles = ((n + 127) / 128) * ((m + p.nt - 1) / p.nt);
-  const int64_t room = p.nt == 64 ? sms : 2 * sms;
   double split = 1e30, pair = 1e30;
   for (int c = 1; c <= kMaxCluster && 2 * c <= 3 * kb; c *= 2) {
-    if (c > 1 && tiles * c > room) break;
-    const double each = 4.0 + 0.39 * (double)((kb + c - 1) / c) + (c > 1 ? join : 0.0) + (c > 4 ? join : 0.0);
-    const double all = 2.0 + (double)(tiles * kb) / 330.0 * (p.nt == 64 ? 1.0 : 0.5);
+    if (c > 1 && tiles * c > 2 * sms) break;
+    const bool two = p.nt == 64 && c > 1 && tiles * c > sms;         // CTAs of one SM
+    const double each = 4.0 + (two ? 1.7 : 0.0) + (two ? 0.48 : 0.39) * (double)((kb + c - 1) / c) +
+                        (c > 1 ? join : 0.0) + (c > 4 ? (two ? 1.6 : 0.4) : 0.0);
+    const double all = 2.0 + (double)tiles * ((double)kb + 2.5) / 330.0 * (p.nt == 64 ? 1.0 : 0.5);
     const double t = each > all ? each : all;
     if (t < split) {
       split = t;
