@@ -13,7 +13,8 @@
 // registers and cross shared memory as bytes (16 KB), written out in whole
 // 128-byte rows.  Measured, 65536 x 2304 bfloat16: rows 69 us (6.5 TB/s), rows and
 // columns 104 us (5.8), square blocks with their transpose 99 us; float32 rows and
-// columns 141 us (6.4).
+// columns 141 us (6.4).  Odd widths or strides are read element by element:
+// 65536 x 2303 rows 206 us and both 263 (bfloat16, 2.2 TB/s), 169 and 237 (float32, 4.5).
 #include "race_api.h"
 #include "race_lowp.cuh"
 
@@ -113,8 +114,11 @@ __device__ __forceinline__ uint2 code_row(const Tile<T>& t, int i, float inv) {
   return code8(v, inv);
 }
 
+// Three CTAs an SM where 80 registers hold a thread's values and codes: float32 by rows
+// and columns takes 122 (square blocks of 21700 x 2303 float32 with their transpose 66 us;
+// 80 with the 94 registers that the compiler takes by itself).
 template <typename T, bool VEC, bool SQUARE, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_quantize(const Args a) {
+__global__ void __launch_bounds__(NT, sizeof(T) == 2 || SQUARE ? 3 : 2) k_quantize(const Args a) {
   __shared__ __align__(16) uint2 tile[COLS ? 128 * 16 : 1];   // [column][8-row group], swizzled
   constexpr int CW = Tile<T>::CW;                              // words of 8 columns' maxima
   __shared__ uint32_t wmax[8][COLS && !SQUARE ? 16 * CW : 1];
