@@ -1,7 +1,8 @@
 """AdamW over all tensors of a model in one launch, with states in 32 or 8 bits.
 
 The reference trains with torch.optim.AdamW; this optimizer has its update rule
-and its arguments.  States live in one allocation each for all parameters,
+and its lr, betas, eps and weight_decay (no amsgrad, maximize, capturable or
+differentiable).  States live in one allocation each for all parameters,
 every tensor starting on a multiple of 128 elements.
 """
 from __future__ import annotations
