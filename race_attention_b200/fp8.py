@@ -259,7 +259,9 @@ class Fp8Linear(nn.Module):
     once for serving; ``release()`` drops that copy.  Training mode ignores it,
     and where the weight has changed since (a loaded state, an optimizer's step,
     another device or type) the next serving call quantises it again.  Writes
-    through ``weight.data`` cannot be seen: call ``hold()`` after them."""
+    through ``weight.data`` cannot be seen: call ``hold()`` after them.  Inputs
+    that ask for a gradient go through the weight itself, in eval mode too; others
+    are served, and the weight gets no gradient from them."""
 
     def __init__(self, in_features: int, out_features: int, device=None, dtype=None):
         super().__init__()
@@ -296,7 +298,8 @@ class Fp8Linear(nn.Module):
         return self
 
     def forward(self, x, out_dtype: Optional[torch.dtype] = None):
-        if self.held is not None and not self.training:
+        if self.held is not None and not self.training and not (
+                torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad):
             if self._held_at != self._version():
                 self.hold()
             return fp8_linear(x, self.held, out_dtype)

@@ -120,3 +120,28 @@ def test_one_row_serves_as_either_kind():
         fp8_linear(x, quantize_fp8(torch.randn(2, 300, device="cuda")))
     with pytest.raises(ValueError, match="scale for each row"):
         fp8_matmul(quantize_fp8(torch.randn(2, 300, device="cuda"), square=True), h)
+
+
+def test_gradients_in_eval_mode():
+    """A held layer passes the gradients that it passes without its copy."""
+    m, x = layer(0), torch.randn(7, 256, device="cuda", requires_grad=True)
+    m.eval()
+    ref = torch.autograd.grad(m(x).square().sum(), (x, m.weight))
+    m.hold()
+    got = torch.autograd.grad(m(x).square().sum(), (x, m.weight))
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    assert not m(x.detach()).requires_grad          # served
+
+
+def test_a_held_decoder_in_eval_mode_has_gradients():
+    from race_attention_b200.block8 import RACEDecoder8
+    torch.manual_seed(0)
+    model = RACEDecoder8(vocab=64, width=128, heads=4, layers=2, device="cuda").eval()
+    tokens = torch.randint(0, 64, (2, 50), device="cuda")
+    model(tokens).float().square().mean().backward()
+    ref = {n: p.grad.clone() for n, p in model.named_parameters()}
+    model.zero_grad()
+    model.hold()
+    model(tokens).float().square().mean().backward()
+    for n, p in model.named_parameters():
+        assert torch.equal(p.grad, ref[n]), n
