@@ -279,9 +279,9 @@ __global__ void __launch_bounds__(threads_of(WPR), WPR == 32 && !VEC && Q ? 1 : 
 // The CTA of the backward pass: eight warps where a warp holds a row, so that few
 // partial sums of dweight remain.
 constexpr int bwd_threads(int wpr) { return wpr == 1 ? 256 : 32 * wpr; }
-// With vector loads the three rows wait in shared memory, STAGES rows deep, each lane
-// copying and reading its own 16 bytes (so no barrier): one row ahead in registers
-// took 171 of them at three spans and left 8 warps an SM.
+// The staged form (can_stage says where): the three rows wait in shared memory, STAGES
+// rows deep, each lane copying and reading its own 16 bytes (so no barrier): one row
+// ahead in registers took 171 of them at three spans and left 8 warps an SM.
 template <typename T, int V, int WPR>
 struct Staged {
   static constexpr int PART = (int)sizeof(T) / 2 * 512;          // bytes of a warp's span: 16 or 32 a lane
